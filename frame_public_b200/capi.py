@@ -51,6 +51,22 @@ class Conv2dParams(Structure):
                                        "stride_w", "pad_h", "pad_w", "groups")]
 
 
+class AttentionParams(Structure):
+    """fb200_attention_params; strides in elements."""
+    _fields_ = [(n, c_int64) for n in ("n_seqs", "heads", "kv_heads", "head_dim", "q_rows", "kv_rows", "max_q",
+                                       "max_kv", "q_token_stride", "q_head_stride", "o_token_stride",
+                                       "o_head_stride", "k_token_stride", "k_head_stride", "v_token_stride",
+                                       "v_head_stride")] + [("scale", c_float), ("causal", c_int), ("dtype", c_int)]
+
+
+class KvCache(Structure):
+    """fb200_kv_cache: pages of keys and values; dtype U8 = e4m3 codes with scale bytes."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p)] + \
+               [(n, c_int64) for n in ("pages", "page_size", "kv_heads", "head_dim", "page_stride", "token_stride",
+                                       "head_stride", "scale_page_stride", "scale_token_stride",
+                                       "scale_head_stride")] + [("dtype", c_int)]
+
+
 # Every exported symbol of include/frame_b200.h: name -> (restype, argtypes)
 _P = c_void_p
 _PP = POINTER(c_void_p)
@@ -122,6 +138,14 @@ SIGNATURES = {
     "fb200_attention_fan_supported": (c_int, [c_int64, c_int64, c_int64, c_int]),
     "fb200_attention_fan": (c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P,
                                     c_int64, _P, c_int64, c_int64, c_int64, c_int64, c_float, c_int, _P]),
+    "fb200_attention_prompt": (c_int, [POINTER(AttentionParams)] + [_P] * 8),
+    "fb200_kv_cache_write": (c_int, [POINTER(KvCache), _P, c_int64, c_int64, _P, c_int64, c_int64, _P, _P, _P,
+                                     c_int64, c_int64, c_int64, c_int, _P]),
+    "fb200_kv_cache_read": (c_int, [POINTER(KvCache), _P, c_int64, c_int64, _P, c_int64, c_int64, _P, _P,
+                                    c_int64, c_int64, c_int64, c_int, _P]),
+    "fb200_attention_paged_workspace": (c_int, [POINTER(AttentionParams), POINTER(KvCache), POINTER(c_size_t)]),
+    "fb200_attention_paged": (c_int, [POINTER(AttentionParams), POINTER(KvCache)] + [_P] * 6 +
+                              [c_int64, _P, c_size_t, _P]),
     "fb200_mamba_scan": (c_int, [_P] * 8 + [c_int64] * 4 + [_P]),
     "fb200_transpose": (c_int, [_P, _P, c_int, _I64P, _I64P, c_int, _P]),
     "fb200_slice": (c_int, [_P, _P, c_int, _I64P, c_int64, c_int64, c_int64, c_int, _P]),
@@ -393,6 +417,37 @@ def attention_fan(q, q_rows, q_ld, k, k_rows, k_ld, v, v_rows, v_ld, o, o_ld, he
     """heads_dev: device pointer of an array of HEAD_DTYPE records (fb200_attention_head)."""
     check(load().fb200_attention_fan(q, q_rows, q_ld, k, k_rows, k_ld, v, v_rows, v_ld, o, o_ld,
                                      heads_dev, n_heads, sq, sk, head_dim, scale, dtype, stream))
+
+
+def attention_prompt(params: AttentionParams, q, k, v, o, cu_q, cu_kv, lse=None, stream=None):
+    """Attention of packed prompts; cu_q, cu_kv: device pointers of int32 row offsets."""
+    check(load().fb200_attention_prompt(byref(params), q, k, v, o, lse, cu_q, cu_kv, stream))
+
+
+def kv_cache_write(cache: KvCache, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, cu_q, kv_len,
+                   block_table, table_stride, n_seqs, rows, dtype, stream=None):
+    check(load().fb200_kv_cache_write(byref(cache), k, k_token_stride, k_head_stride, v, v_token_stride,
+                                      v_head_stride, cu_q, kv_len, block_table, table_stride, n_seqs, rows, dtype,
+                                      stream))
+
+
+def kv_cache_read(cache: KvCache, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, cu_kv,
+                  block_table, table_stride, n_seqs, rows, dtype, stream=None):
+    check(load().fb200_kv_cache_read(byref(cache), k, k_token_stride, k_head_stride, v, v_token_stride,
+                                     v_head_stride, cu_kv, block_table, table_stride, n_seqs, rows, dtype, stream))
+
+
+def attention_paged_workspace(params: AttentionParams, cache: KvCache) -> int:
+    """Bytes of workspace attention_paged needs; zero it once before the first call."""
+    size = c_size_t(0)
+    check(load().fb200_attention_paged_workspace(byref(params), byref(cache), byref(size)))
+    return size.value
+
+
+def attention_paged(params: AttentionParams, cache: KvCache, q, o, cu_q, kv_len, block_table, table_stride, workspace,
+                    workspace_bytes, lse=None, stream=None):
+    check(load().fb200_attention_paged(byref(params), byref(cache), q, o, lse, cu_q, kv_len, block_table,
+                                       table_stride, workspace, workspace_bytes, stream))
 
 
 def transpose(x, out, dims, perm, itemsize, stream=None):

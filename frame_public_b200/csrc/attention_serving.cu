@@ -1,0 +1,210 @@
+// Attention of packed sequences over dense or paged keys and values: one warp per (query row, head).
+#include "kv_cache.cuh"
+
+#include <climits>
+
+namespace fb200 {
+
+int device_status_word(int** dev_ptr);
+
+int check_attention_params(const char* what, const fb200_attention_params* p) {
+  if (p == nullptr) return set_error(FB200_INVALID_ARGUMENT, "%s: null params", what);
+  if (p->n_seqs < 0 || p->n_seqs > INT_MAX - 1 || p->q_rows < 0 || p->q_rows > INT_MAX || p->kv_rows < 0 ||
+      p->kv_rows > INT_MAX || p->max_q < 0 || p->max_kv < 0) {
+    return set_error(FB200_INVALID_ARGUMENT, "%s: a size is negative or past 2^31", what);
+  }
+  if (p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads || p->heads > 65535) {
+    return set_error(FB200_INVALID_ARGUMENT, "%s: heads (%lld) must be a multiple of kv_heads (%lld)", what,
+                     (long long)p->heads, (long long)p->kv_heads);
+  }
+  if (p->dtype != FB200_BF16 && p->dtype != FB200_F16) {
+    return set_error(FB200_UNIMPLEMENTED, "%s: needs bfloat16 or float16 (got dtype %d)", what, p->dtype);
+  }
+  if (p->head_dim < 16 || p->head_dim > 128 || p->head_dim % 16 || p->heads / p->kv_heads > 64) {
+    return set_error(FB200_UNIMPLEMENTED,
+                     "%s: needs head_dim a multiple of 16 up to 128 and at most 64 query heads per kv head (got %lld, %lld)",
+                     what, (long long)p->head_dim, (long long)(p->heads / p->kv_heads));
+  }
+  if (!(p->scale > 0.0f) || p->scale > 3.0e38f) {
+    return set_error(FB200_INVALID_ARGUMENT, "%s: the score scale must be positive and finite", what);
+  }
+  const int64_t strides[4] = {p->q_token_stride, p->q_head_stride, p->o_token_stride, p->o_head_stride};
+  for (int64_t s : strides) {
+    if (s % 8 || s < p->head_dim) {
+      return set_error(FB200_INVALID_ARGUMENT, "%s: strides must be multiples of 8 elements and at least head_dim", what);
+    }
+  }
+  return FB200_OK;
+}
+
+struct Problem {
+  const uint8_t* q;
+  uint8_t* o;
+  float* lse;
+  const uint8_t* k;   // dense keys and values, or null: the cache
+  const uint8_t* v;
+  const int32_t* cu_q;
+  const int32_t* cu_kv;
+  const int32_t* kv_len;
+  int64_t q_token, q_head, o_token, o_head, k_token, k_head, v_token, v_head;
+  int n_seqs, q_rows, kv_rows, heads, group, dim, causal;
+  float scale;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) attention_rows_kernel(Problem p, PagedCache c, bool paged, bool e4m3, int* status) {
+  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (unit >= static_cast<int64_t>(p.q_rows) * p.heads) return;
+  const int row = static_cast<int>(unit / p.heads), h = static_cast<int>(unit % p.heads), hk = h / p.group;
+  const int s = sequence_of_row(p.cu_q, p.n_seqs, row);
+  if (s < 0) return;
+  int q0, lq, k0 = 0, lk;
+  sequence_span(p.cu_q, s, p.q_rows, q0, lq);
+  if (paged) lk = cached_length(p.kv_len[s], c.table_stride, c.page_shift);
+  else sequence_span(p.cu_kv, s, p.kv_rows, k0, lk);
+  const int last = p.causal ? min(lk - 1, row - q0 + lk - lq) : lk - 1;
+  float q[4], acc[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
+  const T* qp = reinterpret_cast<const T*>(p.q) + row * p.q_token + h * p.q_head;
+  for (int i = 0; i < 4; ++i) q[i] = lane + 32 * i < p.dim ? to_f32(qp[lane + 32 * i]) : 0.0f;
+  for (int j = 0; j <= last; ++j) {
+    float ks = 1.0f, vs = 1.0f;
+    int64_t ka, va;
+    const uint8_t *kb = p.k, *vb = p.v;
+    if (paged) {
+      const int page = page_number(c, s, j >> c.page_shift, status);
+      ka = va = token_offset(c, page, j, hk);
+      kb = c.k;
+      vb = c.v;
+      if (e4m3) {
+        const int64_t at = scale_offset(c, page, j, hk);
+        ks = scale_of_byte(c.k_scale[at]);
+        vs = scale_of_byte(c.v_scale[at]);
+      }
+    } else {
+      ka = (k0 + j) * p.k_token + hk * p.k_head;
+      va = (k0 + j) * p.v_token + hk * p.v_head;
+    }
+    float dot = 0.0f, v[4];
+    for (int i = 0; i < 4; ++i) {
+      const int d = lane + 32 * i;
+      float kx = 0.0f;
+      v[i] = 0.0f;
+      if (d < p.dim) {
+        kx = e4m3 ? e4m3x2_to_f32(kb[ka + d]).x : to_f32(reinterpret_cast<const T*>(kb)[ka + d]);
+        v[i] = (e4m3 ? e4m3x2_to_f32(vb[va + d]).x : to_f32(reinterpret_cast<const T*>(vb)[va + d])) * vs;
+      }
+      dot += q[i] * kx;
+    }
+    for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+    const float sc = dot * ks * p.scale, nm = fmaxf(m, sc);
+    const float corr = m == -INFINITY ? 0.0f : expf(m - nm), e = nm == -INFINITY ? 0.0f : expf(sc - nm);
+    m = nm;
+    l = l * corr + e;
+    for (int i = 0; i < 4; ++i) acc[i] = acc[i] * corr + e * v[i];
+  }
+  T* op = reinterpret_cast<T*>(p.o) + row * p.o_token + h * p.o_head;
+  for (int i = 0; i < 4; ++i) {
+    if (lane + 32 * i < p.dim) op[lane + 32 * i] = from_f32<T>(l == 0.0f ? 0.0f : acc[i] / l);
+  }
+  if (p.lse && lane == 0) p.lse[static_cast<int64_t>(row) * p.heads + h] = l == 0.0f ? -INFINITY : m + logf(l);
+}
+
+static Problem make_problem(const fb200_attention_params* p, const void* q, void* o, float* lse, const int32_t* cu_q) {
+  Problem r{};
+  r.q = static_cast<const uint8_t*>(q);
+  r.o = static_cast<uint8_t*>(o);
+  r.lse = lse;
+  r.cu_q = cu_q;
+  r.q_token = p->q_token_stride;
+  r.q_head = p->q_head_stride;
+  r.o_token = p->o_token_stride;
+  r.o_head = p->o_head_stride;
+  r.n_seqs = static_cast<int>(p->n_seqs);
+  r.q_rows = static_cast<int>(p->q_rows);
+  r.kv_rows = static_cast<int>(p->kv_rows);
+  r.heads = static_cast<int>(p->heads);
+  r.group = static_cast<int>(p->heads / p->kv_heads);
+  r.dim = static_cast<int>(p->head_dim);
+  r.causal = p->causal != 0;
+  r.scale = p->scale;
+  return r;
+}
+
+static int launch_rows(const Problem& r, const PagedCache& c, bool paged, bool e4m3, int dtype, cudaStream_t s) {
+  int* status = nullptr;
+  if (int rc = device_status_word(&status)) return rc;
+  const int64_t blocks = (static_cast<int64_t>(r.q_rows) * r.heads + 7) / 8;
+  if (dtype == FB200_BF16) attention_rows_kernel<__nv_bfloat16><<<static_cast<unsigned>(blocks), 256, 0, s>>>(r, c, paged, e4m3, status);
+  else attention_rows_kernel<__half><<<static_cast<unsigned>(blocks), 256, 0, s>>>(r, c, paged, e4m3, status);
+  return after_launch("attention_rows_kernel");
+}
+
+}  // namespace fb200
+
+using namespace fb200;
+
+extern "C" int fb200_attention_prompt(const fb200_attention_params* params, const void* q, const void* k, const void* v,
+                                      void* o, float* lse, const int32_t* cu_q, const int32_t* cu_kv, fb200_stream stream) {
+  if (int rc = check_attention_params("attention_prompt", params)) return rc;
+  const int64_t strides[4] = {params->k_token_stride, params->k_head_stride, params->v_token_stride, params->v_head_stride};
+  for (int64_t s : strides) {
+    if (s % 8 || s < params->head_dim) {
+      return set_error(FB200_INVALID_ARGUMENT, "attention_prompt: strides must be multiples of 8 elements and at least head_dim");
+    }
+  }
+  if (params->n_seqs == 0 || params->q_rows == 0) return FB200_OK;
+  if (!q || !o || !cu_q || !cu_kv || (params->kv_rows > 0 && (!k || !v))) {
+    return set_error(FB200_INVALID_ARGUMENT, "attention_prompt: null argument");
+  }
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)) {
+    return set_error(FB200_INVALID_ARGUMENT, "attention_prompt: q, k, v and o must be 16-byte aligned");
+  }
+  Problem r = make_problem(params, q, o, lse, cu_q);
+  r.k = static_cast<const uint8_t*>(k);
+  r.v = static_cast<const uint8_t*>(v);
+  r.cu_kv = cu_kv;
+  r.k_token = params->k_token_stride;
+  r.k_head = params->k_head_stride;
+  r.v_token = params->v_token_stride;
+  r.v_head = params->v_head_stride;
+  return launch_rows(r, PagedCache{}, false, false, params->dtype, as_stream(stream));
+}
+
+static int check_paged(const char* what, const fb200_attention_params* p, const fb200_kv_cache* c) {
+  if (int rc = check_attention_params(what, p)) return rc;
+  if (int rc = check_kv_cache(what, c, p->dtype)) return rc;
+  if (c->kv_heads != p->kv_heads || c->head_dim != p->head_dim) {
+    return set_error(FB200_INVALID_ARGUMENT, "%s: the cache's heads and head_dim are not the call's", what);
+  }
+  return FB200_OK;
+}
+
+extern "C" int fb200_attention_paged_workspace(const fb200_attention_params* params, const fb200_kv_cache* cache, size_t* bytes) {
+  if (bytes == nullptr) return set_error(FB200_INVALID_ARGUMENT, "attention_paged_workspace: null out pointer");
+  *bytes = 0;
+  return check_paged("attention_paged_workspace", params, cache);
+}
+
+extern "C" int fb200_attention_paged(const fb200_attention_params* params, const fb200_kv_cache* cache, const void* q, void* o,
+                                     float* lse, const int32_t* cu_q, const int32_t* kv_len, const int32_t* block_table,
+                                     int64_t table_stride, void* workspace, size_t workspace_bytes, fb200_stream stream) {
+  if (int rc = check_paged("attention_paged", params, cache)) return rc;
+  if (table_stride < 0) return set_error(FB200_INVALID_ARGUMENT, "attention_paged: negative table stride");
+  if (params->n_seqs == 0 || params->q_rows == 0) return FB200_OK;
+  if (!q || !o || !cu_q || !kv_len || (table_stride > 0 && !block_table)) {
+    return set_error(FB200_INVALID_ARGUMENT, "attention_paged: null argument");
+  }
+  if (cache->pages == 0 && table_stride > 0) return set_error(FB200_INVALID_ARGUMENT, "attention_paged: a cache without pages");
+  if (!aligned16(q) || !aligned16(o)) return set_error(FB200_INVALID_ARGUMENT, "attention_paged: q and o must be 16-byte aligned");
+  size_t need = 0;
+  if (int rc = fb200_attention_paged_workspace(params, cache, &need)) return rc;
+  if (workspace_bytes < need || (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256))) {
+    return set_error(FB200_INVALID_ARGUMENT, "attention_paged: needs a 256-byte aligned workspace of %zu bytes (got %zu)", need, workspace_bytes);
+  }
+  PagedCache c;
+  if (int rc = make_paged_cache(cache, block_table, table_stride, &c)) return rc;
+  Problem r = make_problem(params, q, o, lse, cu_q);
+  r.kv_len = kv_len;
+  return launch_rows(r, c, true, cache->dtype == FB200_U8, params->dtype, as_stream(stream));
+}

@@ -408,6 +408,90 @@ FB200_API int fb200_attention_fan(const void* q_base, int64_t q_rows, int64_t q_
                                   int64_t o_ld, const fb200_attention_head* heads_dev,
                                   int64_t n_heads, int64_t sq, int64_t sk, int64_t head_dim,
                                   float scale, int dtype, fb200_stream stream);
+/* ---- attention for serving: packed prompts, a paged key/value cache, new tokens over it --------
+ * NEW ops (the reference has no mask, no cache and no ragged batch; its attention is the fan above).
+ * A batch is n_seqs sequences.  Query rows are packed: sequence s owns rows cu_q[s] .. cu_q[s+1]-1
+ * of q and o (cu_q: n_seqs + 1 device int32, not decreasing); rows outside every sequence are
+ * neither read nor written.  With Lq query rows and Lk keys, query i of a sequence sees key j when
+ * j < Lk and, if `causal`, j <= i + Lk - Lq (the last query sees every key).  For query head h:
+ *   O = softmax(scale * Q_h K_{h'}^T over the keys seen) V_{h'},   h' = h / (heads / kv_heads),
+ * a row that sees no key is all zeros (its lse -infinity).  Products and softmax statistics are
+ * fp32; probabilities are rounded to 16 bits before the second product (as in attention_fan), O once
+ * at the store.  lse (optional, fp32 [q_rows, heads]): log of the row's sum of exp(scale * score).
+ * A key that a row does not see does not reach it, whatever its K holds; in 16-bit V a NaN or an
+ * infinity of a later key of the SAME sequence may reach earlier rows of its 128-key tile.
+ * Layouts: element strides per token and per head, head_dim contiguous; every base 16-byte aligned,
+ * every stride a multiple of 8 elements (16 for e4m3 codes).  dtype BF16 or F16; head_dim a
+ * multiple of 16 up to 128; heads a multiple of kv_heads, heads / kv_heads <= 64.  Anything else
+ * is FB200_UNIMPLEMENTED or FB200_INVALID_ARGUMENT.  q_rows and the other extents bound every access:
+ * offsets and lengths that leave them are cut to them.  All pointers belong to the current device. */
+typedef struct fb200_attention_params {
+  int64_t n_seqs, heads, kv_heads, head_dim;
+  int64_t q_rows;    /* rows of q and o */
+  int64_t kv_rows;   /* prompt only: rows of k and v */
+  int64_t max_q;     /* no sequence has more query rows (more are not computed: kernel status 322) */
+  int64_t max_kv;    /* no sequence has more keys: for scheduling only */
+  int64_t q_token_stride, q_head_stride, o_token_stride, o_head_stride;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;   /* prompt only */
+  float scale;       /* > 0 */
+  int causal;
+  int dtype;
+} fb200_attention_params;
+/* A paged cache: token t of a sequence lies in page block_table[s][t / page_size], at place
+ * t % page_size.  k and v share the strides (elements of `dtype`).  dtype: BF16 / F16, or U8 for
+ * e4m3 codes with one scale per (token, kv head): byte b stands for 2^(b - 127), and the values are
+ * code * 2^(b - 127); b = 255 makes the whole token-head NaN.  page_size a power of two from 8 up. */
+typedef struct fb200_kv_cache {
+  void* k;
+  void* v;
+  uint8_t* k_scale;  /* U8 only, else NULL */
+  uint8_t* v_scale;
+  int64_t pages, page_size, kv_heads, head_dim;
+  int64_t page_stride, token_stride, head_stride;
+  int64_t scale_page_stride, scale_token_stride, scale_head_stride;
+  int dtype;
+} fb200_kv_cache;
+/* Causal (or full) attention of whole prompts.  k, v: [kv_rows, kv_heads, head_dim], sequence s
+ * owns rows cu_kv[s] .. cu_kv[s+1]-1 (cu_kv may be cu_q; more keys than queries: a dense prefix).
+ * o must not overlap q, k or v. */
+FB200_API int fb200_attention_prompt(const fb200_attention_params* params, const void* q, const void* k,
+                                     const void* v, void* o, float* lse, const int32_t* cu_q,
+                                     const int32_t* cu_kv, fb200_stream stream);
+/* Stores the keys and values of new tokens: row i of sequence s (cu_q as above, `rows` rows of k and
+ * v) goes to token kv_len[s] - Lq + i; kv_len (device int32) counts the new tokens already.  A 16-bit
+ * cache takes the numbers as they are (its dtype must be `dtype`).  An e4m3 cache takes, per token
+ * and head, the smallest 2^e with e >= -126 and max|x| <= 448 * 2^e, and x * 2^-e rounded to nearest
+ * even; a token-head with an infinity or a NaN is stored as scale byte 255 and codes 0.  block_table:
+ * device int32 [n_seqs, table_stride].  A page number outside the cache, or a token outside the
+ * table, is skipped and recorded as kernel status 321 / 322.  Two tokens of one call must not share
+ * a place (pages shared by sequences hold whole prefixes, which are not written again). */
+FB200_API int fb200_kv_cache_write(const fb200_kv_cache* cache, const void* k, int64_t k_token_stride,
+                                   int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                                   int64_t v_head_stride, const int32_t* cu_q, const int32_t* kv_len,
+                                   const int32_t* block_table, int64_t table_stride, int64_t n_seqs,
+                                   int64_t rows, int dtype, fb200_stream stream);
+/* The first cu_kv[s+1] - cu_kv[s] cached tokens of every sequence as rows cu_kv[s] .. of dense k and
+ * v ([rows, kv_heads, head_dim] of `dtype`).  e4m3 values are exact in bfloat16 and rounded once to
+ * float16.  Bad pages as in the write (their rows stay as they were). */
+FB200_API int fb200_kv_cache_read(const fb200_kv_cache* cache, void* k, int64_t k_token_stride,
+                                  int64_t k_head_stride, void* v, int64_t v_token_stride,
+                                  int64_t v_head_stride, const int32_t* cu_kv, const int32_t* block_table,
+                                  int64_t table_stride, int64_t n_seqs, int64_t rows, int dtype,
+                                  fb200_stream stream);
+/* New tokens (one per sequence in a decoding step, a chunk of a prompt, drafted tokens) over the
+ * cache, which holds them already (fb200_kv_cache_write).  kv_len: device int32 [n_seqs]; the cache's
+ * dtype is params->dtype or U8.  Long caches are split over the SMs when there are few rows; the
+ * parts meet in `workspace` (fb200_attention_paged_workspace bytes, 256-byte aligned), which must be
+ * zero before its first use, may be used by any later call on the same stream (every call leaves
+ * the part that has to be zero so), and must not be shared by calls that overlap.  The parts are
+ * joined in a fixed order: results do not depend on timing.  A key on a page number outside the cache
+ * is taken from page 0 and recorded as kernel status 321. */
+FB200_API int fb200_attention_paged_workspace(const fb200_attention_params* params,
+                                              const fb200_kv_cache* cache, size_t* bytes);
+FB200_API int fb200_attention_paged(const fb200_attention_params* params, const fb200_kv_cache* cache,
+                                    const void* q, void* o, float* lse, const int32_t* cu_q,
+                                    const int32_t* kv_len, const int32_t* block_table, int64_t table_stride,
+                                    void* workspace, size_t workspace_bytes, fb200_stream stream);
 /* NEW op (no reference counterpart): the Mamba SSM scan with un-materialised operands, fp32.
  * u, delta, z, y: [batch, len, dm]; A: [dm, nstate]; B, C: [batch, len, nstate]; D: [dm];
  * z may be NULL.  h[n] = exp(delta*A[d,n])*h[n] + delta*B[n]*u; y = sum_n C[n]*h[n] + D[d]*u;
