@@ -1,5 +1,5 @@
 // Attention of packed sequences over dense or paged keys and values: one warp per (query row, head).
-#include "kv_cache.cuh"
+#include "attention_serving.cuh"
 
 #include <climits>
 
@@ -9,9 +9,9 @@ int device_status_word(int** dev_ptr);
 
 int check_attention_params(const char* what, const fb200_attention_params* p) {
   if (p == nullptr) return set_error(FB200_INVALID_ARGUMENT, "%s: null params", what);
-  if (p->n_seqs < 0 || p->n_seqs > INT_MAX - 1 || p->q_rows < 0 || p->q_rows > INT_MAX || p->kv_rows < 0 ||
-      p->kv_rows > INT_MAX || p->max_q < 0 || p->max_kv < 0) {
-    return set_error(FB200_INVALID_ARGUMENT, "%s: a size is negative or past 2^31", what);
+  if (p->n_seqs < 0 || p->n_seqs > INT_MAX - 1 || p->q_rows < 0 || p->q_rows > kMostTokens || p->kv_rows < 0 ||
+      p->kv_rows > kMostTokens || p->max_q < 0 || p->max_kv < 0) {
+    return set_error(FB200_INVALID_ARGUMENT, "%s: a size is negative or past 2^30", what);
   }
   if (p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads || p->heads > 65535) {
     return set_error(FB200_INVALID_ARGUMENT, "%s: heads (%lld) must be a multiple of kv_heads (%lld)", what,
@@ -37,22 +37,8 @@ int check_attention_params(const char* what, const fb200_attention_params* p) {
   return FB200_OK;
 }
 
-struct Problem {
-  const uint8_t* q;
-  uint8_t* o;
-  float* lse;
-  const uint8_t* k;   // dense keys and values, or null: the cache
-  const uint8_t* v;
-  const int32_t* cu_q;
-  const int32_t* cu_kv;
-  const int32_t* kv_len;
-  int64_t q_token, q_head, o_token, o_head, k_token, k_head, v_token, v_head;
-  int n_seqs, q_rows, kv_rows, heads, group, dim, causal;
-  float scale;
-};
-
 template <typename T>
-__global__ void __launch_bounds__(256) attention_rows_kernel(Problem p, PagedCache c, bool paged, bool e4m3, int* status) {
+__global__ void __launch_bounds__(256) attention_rows_kernel(ServingProblem p, PagedCache c, bool paged, bool e4m3, int* status) {
   const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (unit >= static_cast<int64_t>(p.q_rows) * p.heads) return;
@@ -110,8 +96,8 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(Problem p, PagedCac
   if (p.lse && lane == 0) p.lse[static_cast<int64_t>(row) * p.heads + h] = l == 0.0f ? -INFINITY : m + logf(l);
 }
 
-static Problem make_problem(const fb200_attention_params* p, const void* q, void* o, float* lse, const int32_t* cu_q) {
-  Problem r{};
+static ServingProblem make_problem(const fb200_attention_params* p, const void* q, void* o, float* lse, const int32_t* cu_q) {
+  ServingProblem r{};
   r.q = static_cast<const uint8_t*>(q);
   r.o = static_cast<uint8_t*>(o);
   r.lse = lse;
@@ -125,13 +111,16 @@ static Problem make_problem(const fb200_attention_params* p, const void* q, void
   r.kv_rows = static_cast<int>(p->kv_rows);
   r.heads = static_cast<int>(p->heads);
   r.group = static_cast<int>(p->heads / p->kv_heads);
+  r.kv_heads = static_cast<int>(p->kv_heads);
   r.dim = static_cast<int>(p->head_dim);
+  r.max_q = static_cast<int>(p->max_q < p->q_rows ? p->max_q : p->q_rows);
+  r.dtype = p->dtype;
   r.causal = p->causal != 0;
   r.scale = p->scale;
   return r;
 }
 
-static int launch_rows(const Problem& r, const PagedCache& c, bool paged, bool e4m3, int dtype, cudaStream_t s) {
+static int launch_rows(const ServingProblem& r, const PagedCache& c, bool paged, bool e4m3, int dtype, cudaStream_t s) {
   int* status = nullptr;
   if (int rc = device_status_word(&status)) return rc;
   const int64_t blocks = (static_cast<int64_t>(r.q_rows) * r.heads + 7) / 8;
@@ -160,7 +149,7 @@ extern "C" int fb200_attention_prompt(const fb200_attention_params* params, cons
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)) {
     return set_error(FB200_INVALID_ARGUMENT, "attention_prompt: q, k, v and o must be 16-byte aligned");
   }
-  Problem r = make_problem(params, q, o, lse, cu_q);
+  ServingProblem r = make_problem(params, q, o, lse, cu_q);
   r.k = static_cast<const uint8_t*>(k);
   r.v = static_cast<const uint8_t*>(v);
   r.cu_kv = cu_kv;
@@ -168,7 +157,7 @@ extern "C" int fb200_attention_prompt(const fb200_attention_params* params, cons
   r.k_head = params->k_head_stride;
   r.v_token = params->v_token_stride;
   r.v_head = params->v_head_stride;
-  return launch_rows(r, PagedCache{}, false, false, params->dtype, as_stream(stream));
+  return launch_attention_tiles(r, nullptr, nullptr, as_stream(stream));
 }
 
 static int check_paged(const char* what, const fb200_attention_params* p, const fb200_kv_cache* c) {
@@ -204,7 +193,8 @@ extern "C" int fb200_attention_paged(const fb200_attention_params* params, const
   }
   PagedCache c;
   if (int rc = make_paged_cache(cache, block_table, table_stride, &c)) return rc;
-  Problem r = make_problem(params, q, o, lse, cu_q);
+  ServingProblem r = make_problem(params, q, o, lse, cu_q);
   r.kv_len = kv_len;
+  if (cache->dtype != FB200_U8 && params->max_q * r.group > 16) return launch_attention_tiles(r, &c, cache, as_stream(stream));
   return launch_rows(r, c, true, cache->dtype == FB200_U8, params->dtype, as_stream(stream));
 }

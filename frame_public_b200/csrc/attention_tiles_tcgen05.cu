@@ -1,0 +1,473 @@
+// Attention of packed sequences on the tensor cores: 128 query rows at a time over tiles of 128 keys,
+//   S = Q K^T,  m' = max(m, rowmax S),  P = 2^(c S - c m'),  l = l 2^(c m - c m') + rowsum P,
+//   O = O 2^(c m - c m') + P V,  result O / l,   c = scale * log2(e),
+// one pass over the keys with the running maximum and sum in fp32.
+//
+// A row is a (token, query head) pair: the query heads that share a kv head lie next to each other in
+// the tile (128 / group tokens of `group` heads), so a key tile is read once for all of them and short
+// chunks of new tokens still fill the tensor core's 128 rows.
+//
+// A CTA holds two such tiles ("stages") and walks the keys both see.  Roles:
+//   warps 0-3, 4-7   softmax of stage 0 and 1, one thread per row = TMEM lane: tcgen05.ld of the row's
+//                    128 scores, maximum, exponentials, tcgen05.st of P (16 bit) over S
+//   warp 8           every tcgen05.mma: S_s = Q_s K^T (both operands in shared memory), O_s += P_s V with
+//                    P as the A operand in TMEM, so P never passes through shared memory
+//   warp 9           TMA: Q once, K and V tiles through a ring; a paged cache one box per page
+// While the threads of one stage compute exponentials the tensor core works on the other one.  TMEM:
+// S0, S1 (128 columns each, P over the first 64), O0, O1.
+// O is only rescaled when a row's maximum grew by more than 2^8 since the last time (the exponents stay
+// below 2^8 then, which fp32 sums and 16-bit P hold as well as values up to 1).
+//
+// Bounds: 4 * pairs * head_dim FLOP against the tensor pipe; one exponential per pair against the
+// XU pipe (16 per SM and cycle: 1024 cycles for a 128 x 128 tile whose two products take 512 to 1024).
+#include <cuda.h>
+
+#include "attention_serving.cuh"
+#include "sm100_ptx.cuh"
+
+namespace fb200 {
+
+int make_tmap_4d(CUtensorMap* map, const void* ptr, int dtype, const int64_t (&dims)[4], const int64_t (&stride_bytes)[3],
+                 const int (&box)[4]);
+int device_status_word(int** dev_ptr);
+
+using namespace sm100;
+
+constexpr int kTileRows = 128;
+constexpr int kTileKeys = 128;
+constexpr int kTilesThreads = 320;
+constexpr int kSpanBytes = kTileRows * 128;   // 128 rows of 64 16-bit elements
+constexpr float kRescaleStep = 8.0f;          // log2 of the growth of a row's maximum that O follows at once
+
+enum TilesFault : int {
+  kFaultTilesQuery = 331,
+  kFaultTilesKeys = 332,
+  kFaultTilesScores = 333,
+  kFaultTilesProbs = 334,
+  kFaultTilesRing = 335,
+  kFaultTilesOutput = 336,
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T> __device__ __forceinline__ uint32_t pack_pair(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// A CTA's share of the work.
+struct TilesItem {
+  int seq, block, q0, lq, k0, lk;
+};
+
+// Keys that the block ending before token `end` sees.
+__device__ __forceinline__ int keys_seen(int causal, int end, int lq, int lk) {
+  return causal ? max(0, min(lk, end + lk - lq)) : lk;
+}
+
+// Item `rank` of the blocks of `tokens` query tokens of all sequences in order of falling cost (tiles of
+// keys): the long ones start first, so that the last CTAs to run are short ones.  The number of blocks
+// that cost more than c tiles is a closed form per sequence; a binary search over c finds the cost of
+// the rank, a scan over the sequences the block.  Run by one warp; returns false past the last item.
+template <bool PAGED>
+__device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int rank, int tokens, TilesItem& item,
+                          int* status) {
+  const int lane = threadIdx.x & 31;
+  // blocks of sequence (lq, lk) that see more than 128 * c keys
+  auto above = [&](int lq, int lk, int c) {
+    const int blocks = (lq + tokens - 1) / tokens;
+    if (c < 0) return blocks;
+    if (lk <= c * kTileKeys) return 0;
+    if (!p.causal) return blocks;
+    const int y = c * kTileKeys - lk + lq;   // blocks that end at or before token y see no more
+    return blocks - max(0, min(y >= 0 ? y / tokens : 0, blocks - 1));
+  };
+  auto total = [&](int c, int& longest) {
+    int sum = 0, most = 0;
+    for (int s = lane; s < p.n_seqs; s += 32) {
+      int q0, lq, k0, lk;
+      serving_lengths<PAGED>(p, cache, s, q0, lq, k0, lk);
+      sum += above(lq, lk, c);
+      most = max(most, lk);
+      if (rank == 0 && c < 0 && lq > p.max_q) record_fault(status, kFaultBadLength);
+    }
+    longest = __reduce_max_sync(0xffffffffu, most);
+    return __reduce_add_sync(0xffffffffu, sum);
+  };
+  int longest = 0;
+  if (rank >= total(-1, longest)) return false;
+  int lo = -1, hi = (longest + kTileKeys - 1) / kTileKeys;   // total(lo) > rank >= total(hi)
+  int below = 0, ignored;                                    // total(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1, n = total(mid, ignored);
+    if (n > rank) lo = mid;
+    else { hi = mid; below = n; }
+  }
+  // items of cost hi exactly, in sequence order: `rank - below` of them lie before this one
+  int left = rank - below;
+  for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
+    const int s = s0 + lane;
+    int q0 = 0, lq = 0, k0 = 0, lk = 0, n = 0, more = 0;
+    if (s < p.n_seqs) {
+      serving_lengths<PAGED>(p, cache, s, q0, lq, k0, lk);
+      more = above(lq, lk, hi);
+      n = above(lq, lk, hi - 1) - more;
+    }
+    int upto = n;   // inclusive scan
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += x;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, upto > left);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int blocks = (lq + tokens - 1) / tokens;
+      const int block = blocks - more - n + (left - (upto - n));
+      item.seq = s0 + src;
+      item.block = __shfl_sync(0xffffffffu, block, src);
+      item.q0 = __shfl_sync(0xffffffffu, q0, src);
+      item.lq = __shfl_sync(0xffffffffu, lq, src);
+      item.k0 = __shfl_sync(0xffffffffu, k0, src);
+      item.lk = __shfl_sync(0xffffffffu, lk, src);
+      return true;
+    }
+    left -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return false;
+}
+
+template <typename T, int SPANS, bool PAGED>
+__global__ void __launch_bounds__(kTilesThreads, 1)
+attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                       const __grid_constant__ CUtensorMap tmap_v, const ServingProblem p, const PagedCache cache,
+                       int tile_tokens, int box_keys, uint32_t fmt, int* status) {
+  constexpr int kSlotBytes = SPANS * kSpanBytes;
+  constexpr int kSlots = SPANS == 2 ? 5 : 8;
+  constexpr uint32_t kTmemO = 2 * kTileKeys;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - raw_addr);
+  const uint32_t q_s = base, ring = base + 2 * kSlotBytes, bars = ring + kSlots * kSlotBytes;
+  const uint32_t bar_q = bars, full = bars + 8, freed = full + 8 * kSlots, bar_s = freed + 8 * kSlots, bar_p = bar_s + 16,
+                 bar_o = bar_p + 16, tmem_slot = bar_o + 16;
+  uint8_t* const after = base_ptr + (tmem_slot - base);
+  volatile uint32_t* const tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(after);
+  TilesItem* const item_ptr = reinterpret_cast<TilesItem*>(after + 16);
+  int* const found_ptr = reinterpret_cast<int*>(after + 16 + sizeof(TilesItem));
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int head = blockIdx.x % p.kv_heads;
+  if (warp == 0) {
+    TilesItem it;
+    const bool found = find_item<PAGED>(p, cache, blockIdx.x / p.kv_heads, 2 * tile_tokens, it, status);
+    if (lane == 0) {
+      if (found) *item_ptr = it;
+      *found_ptr = found;
+    }
+  } else if (warp == 8 && lane == 0) {
+    mbar_init(bar_q, 1);
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(freed + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_s + 8 * i, 1);
+      mbar_init(bar_p + 8 * i, 4);
+      mbar_init(bar_o + 8 * i, 1);
+    }
+    mbar_fence_init();
+  } else if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tcgen05_fence_before_sync();
+  __syncthreads();
+  tcgen05_fence_after_sync();
+  const uint32_t tmem = *tmem_slot_ptr;
+  const TilesItem item = *item_ptr;
+  const bool work = *found_ptr != 0;
+  const int token0 = item.block * 2 * tile_tokens;
+  int tiles[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int first = token0 + s * tile_tokens;
+    tiles[s] = work && first < item.lq
+                   ? (keys_seen(p.causal, min(item.lq, first + tile_tokens), item.lq, item.lk) + kTileKeys - 1) / kTileKeys
+                   : 0;
+  }
+  const int most = max(tiles[0], tiles[1]);   // stage 1's rows come later: it sees as many, unless it has none
+
+  if (warp == 9) {
+    // ---- copies ----------------------------------------------------------------------------------
+    if (most > 0) {
+      if (lane == 0) {
+        const int live_stages = (tiles[0] > 0) + (tiles[1] > 0);
+        mbar_arrive_expect_tx(bar_q, static_cast<uint32_t>(live_stages * tile_tokens * p.group * 128 * SPANS));
+        for (int s = 0; s < 2; ++s) {
+          if (tiles[s] == 0) continue;
+          for (int x = 0; x < SPANS; ++x) {
+            tma_load_4d(q_s + s * kSlotBytes + x * kSpanBytes, &tmap_q, bar_q, x * 64, 0, item.q0 + token0 + s * tile_tokens, head);
+          }
+        }
+      }
+      __syncwarp();
+      bool live = true;
+      for (int n = 0; live && n < 2 * most; ++n) {   // K and V of tile n / 2 in turn
+        const int j = n >> 1, slot = n % kSlots, use = n / kSlots;
+        const uint32_t dst = ring + slot * kSlotBytes, bar = full + 8 * slot;
+        const void* map = (n & 1) ? static_cast<const void*>(&tmap_v) : &tmap_k;
+        const int key = j * kTileKeys + lane * box_keys;
+        const bool mine = lane * box_keys < kTileKeys && (!PAGED || key < item.lk);
+        const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
+        int page = 0, row = item.k0 + key;
+        if (PAGED && mine) {
+          page = page_number(cache, item.seq, key >> cache.page_shift, status);
+          row = key & ((1 << cache.page_shift) - 1);
+        }
+        if (use > 0) live = mbar_wait_warp(freed + 8 * slot, (use - 1) & 1, status, kFaultTilesRing);
+        if (!live) break;
+        if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(boxes * box_keys * 128 * SPANS));
+        __syncwarp();
+        if (mine) {
+          for (int x = 0; x < SPANS; ++x) {
+            tma_load_4d(dst + x * kSpanBytes + lane * box_keys * 128, map, bar, x * 64, row, head, page);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 8) {
+    // ---- products --------------------------------------------------------------------------------
+    if (most > 0) {
+      const int k_steps = p.dim / 16;
+      const uint32_t idesc_s = make_instr_desc(fmt, 0, 0, kTileRows, kTileKeys);
+      const uint32_t idesc_o = make_instr_desc(fmt, 0, 1, kTileRows, static_cast<uint32_t>(p.dim));
+      const uint64_t q_desc = make_smem_desc_sw128(q_s, 16, 1024);
+      const uint64_t k_desc = make_smem_desc_sw128(ring, 16, 1024);
+      const uint64_t v_desc = make_smem_desc(ring, kSpanBytes, 1024, kLayoutSw128);
+      bool live = mbar_wait_warp(bar_q, 0, status, kFaultTilesQuery);
+      auto scores = [&](int s, int j) {
+        const int n = 2 * j, slot = n % kSlots;
+        live = live && mbar_wait_warp(full + 8 * slot, (n / kSlots) & 1, status, kFaultTilesKeys);
+        if (!live) return;
+        tcgen05_fence_after_sync();
+        const uint64_t a = q_desc + static_cast<uint64_t>(s * kSlotBytes / 16), b = k_desc + static_cast<uint64_t>(slot * kSlotBytes / 16);
+        for (int k = 0; k < k_steps; ++k) {
+          const uint64_t at = static_cast<uint64_t>((k >> 2) * (kSpanBytes / 16) + (k & 3) * 2);
+          mma_f16_elect(tmem + s * kTileKeys, a + at, b + at, idesc_s, k > 0 ? 1u : 0u);
+        }
+        mma_commit_elect(bar_s + 8 * s);
+        if (s == 1 || j >= tiles[1]) mma_commit_elect(freed + 8 * slot);   // the last reader
+      };
+      auto values = [&](int s, int j) {
+        const int n = 2 * j + 1, slot = n % kSlots;
+        live = live && mbar_wait_warp(full + 8 * slot, (n / kSlots) & 1, status, kFaultTilesKeys);
+        live = live && mbar_wait_warp(bar_p + 8 * s, j & 1, status, kFaultTilesProbs);
+        if (!live) return;
+        const int there = item.lk - j * kTileKeys;
+        if (there < kTileKeys && (s == 0 || j >= tiles[0])) {
+          // Rows behind the last key hold another sequence's values or none: their P is 0, but 0 times a
+          // NaN is not.
+          for (int i = lane; i < (kTileKeys - there) * 8 * SPANS; i += 32) {
+            const int row = there + (i >> 3) % (kTileKeys - there), span = (i >> 3) / (kTileKeys - there);
+            *reinterpret_cast<uint4*>(base_ptr + (ring - base) + slot * kSlotBytes + span * kSpanBytes + row * 128 + (i & 7) * 16) =
+                make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        tcgen05_fence_after_sync();
+        const uint64_t b = v_desc + static_cast<uint64_t>(slot * kSlotBytes / 16);
+#pragma unroll
+        for (int k = 0; k < kTileKeys / 16; ++k) {
+          mma_f16_ts_elect(tmem + kTmemO + s * (SPANS * 64), tmem + s * kTileKeys + k * 8, b + k * 128, idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+        }
+        if (s == 1 || j >= tiles[1]) mma_commit_elect(freed + 8 * slot);
+        if (j + 1 == tiles[s]) mma_commit_elect(bar_o + 8 * s);
+      };
+      for (int s = 0; s < 2; ++s) {
+        if (tiles[s] > 0) scores(s, 0);
+      }
+      for (int j = 0; live && j < most; ++j) {
+        for (int s = 0; s < 2; ++s) {
+          if (j < tiles[s]) values(s, j);
+          if (j + 1 < tiles[s]) scores(s, j + 1);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax ---------------------------------------------------------------------------------
+    const int s = warp >> 2, row = threadIdx.x & 127;
+    const int in_tile = row / p.group, token = token0 + s * tile_tokens + in_tile;
+    const int h = head * p.group + row - in_tile * p.group;
+    const bool there = work && in_tile < tile_tokens && token < item.lq;
+    const int limit = there ? keys_seen(p.causal, token + 1, item.lq, item.lk) : 0;   // keys this row sees
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t t_s = lanes + s * kTileKeys, t_o = lanes + kTmemO + s * (SPANS * 64);
+    const float c = p.scale * 1.4426950408889634f;
+    float m = -INFINITY, l = 0.0f;
+    bool live = true;
+    for (int j = 0; j < tiles[s]; ++j) {
+      live = mbar_wait_warp(bar_s + 8 * s, j & 1, status, kFaultTilesScores);
+      if (!live) break;
+      tcgen05_fence_after_sync();
+      uint32_t r[4][32];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_s + i * 32, r[i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_ld_wait(r[i]);
+      const int visible = limit - j * kTileKeys;
+      if (__any_sync(0xffffffffu, visible < kTileKeys)) {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) {
+          if (i >= visible) r[i >> 5][i & 31] = 0xFF800000u;   // -inf
+        }
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 128; i += 2) {
+        top[(i >> 1) & 3] = fmaxf(top[(i >> 1) & 3], fmaxf(__uint_as_float(r[i >> 5][i & 31]), __uint_as_float(r[i >> 5][(i & 31) + 1])));
+      }
+      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      if (j == 0) {
+        m = mx;
+      } else if (__any_sync(0xffffffffu, (mx - m) * c > kRescaleStep)) {   // -inf - -inf compares false
+        // The scores of this tile are there, so the products of the previous ones into O are done too.
+        const float next = fmaxf(m, mx);
+        const float f = next == -INFINITY ? 1.0f : ex2((m - next) * c);
+        m = next;
+        l *= f;
+        for (int i = 0; i < p.dim; i += 16) {
+          uint32_t x[16];
+          tmem_ld_32x32b_x16(t_o + i, x);
+          tmem_ld_wait(x);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+          tmem_st_32x32b_x16(t_o + i, x);
+        }
+      }
+      const float mc = m == -INFINITY ? 0.0f : m * c;
+      float2 sum = make_float2(0.0f, 0.0f);
+      const float2 c2 = make_float2(c, c), nm2 = make_float2(-mc, -mc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t out[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[i][e]), __uint_as_float(r[i][e + 1])), c2, nm2);
+          const float e0 = ex2(x.x), e1 = ex2(x.y);
+          sum = __fadd2_rn(sum, make_float2(e0, e1));
+          out[e >> 1] = pack_pair<T>(e0, e1);
+        }
+        tmem_st_32x32b_x16(t_s + i * 16, out);
+      }
+      l += sum.x + sum.y;
+      tmem_st_wait();
+      tcgen05_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_p + 8 * s);
+    }
+    const bool any = tiles[s] > 0;
+    if (any && live) live = mbar_wait_warp(bar_o + 8 * s, 0, status, kFaultTilesOutput);
+    if (live) {
+      tcgen05_fence_after_sync();
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      T* const dst = reinterpret_cast<T*>(p.o) + static_cast<int64_t>(item.q0 + token) * p.o_token + h * p.o_head;
+      for (int i = 0; i < p.dim; i += 16) {
+        uint32_t x[16];
+        if (any) {
+          tmem_ld_32x32b_x16(t_o + i, x);
+          tmem_ld_wait(x);
+        }
+        if (there) {
+          uint32_t out[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            out[e] = l == 0.0f ? 0u : pack_pair<T>(__uint_as_float(x[2 * e]) * inv, __uint_as_float(x[2 * e + 1]) * inv);
+          }
+          *reinterpret_cast<uint4*>(dst + i) = make_uint4(out[0], out[1], out[2], out[3]);
+          *reinterpret_cast<uint4*>(dst + i + 8) = make_uint4(out[4], out[5], out[6], out[7]);
+        }
+      }
+      if (there && p.lse != nullptr) {
+        p.lse[static_cast<int64_t>(item.q0 + token) * p.heads + h] = l == 0.0f ? -INFINITY : m * p.scale + logf(l);
+      }
+    }
+  }
+  tcgen05_fence_before_sync();
+  __syncthreads();
+  if (warp == 9) {
+    __syncwarp();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Blocks of `tokens` query tokens there can be.
+static int64_t most_blocks(const ServingProblem& p, int64_t tokens) {
+  const int64_t by_rows = p.q_rows / tokens + p.n_seqs;
+  const int64_t by_seq = static_cast<int64_t>(p.n_seqs) * ((p.max_q + tokens - 1) / tokens);
+  return by_rows < by_seq ? by_rows : by_seq;
+}
+
+int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, const fb200_kv_cache* desc, cudaStream_t stream) {
+  const int tile_tokens = kTileRows / p.group;
+  const int64_t grid = most_blocks(p, 2 * tile_tokens) * p.kv_heads;
+  if (grid > 0x7fffffff) return set_error(FB200_INVALID_ARGUMENT, "attention: too many tiles");
+  if (grid == 0) return FB200_OK;
+  const int spans = p.dim > 64 ? 2 : 1;
+  CUtensorMap tq, tk, tv;
+  const int64_t qd[4] = {p.dim, p.group, p.q_rows, p.kv_heads}, qs[3] = {p.q_head * 2, p.q_token * 2, p.q_head * p.group * 2};
+  const int qb[4] = {64, p.group, tile_tokens, 1};
+  if (int rc = make_tmap_4d(&tq, p.q, p.dtype, qd, qs, qb)) return rc;
+  int box_keys = kTileKeys;
+  if (cache != nullptr) {
+    const int64_t page = int64_t(1) << cache->page_shift;
+    if (page < box_keys) box_keys = static_cast<int>(page);
+    const int64_t d[4] = {p.dim, page, p.kv_heads, cache->pages > 0 ? cache->pages : 1};
+    const int64_t st[3] = {cache->token_stride * 2, cache->head_stride * 2, cache->page_stride * 2};
+    const int b[4] = {64, box_keys, 1, 1};
+    if (int rc = make_tmap_4d(&tk, cache->pages > 0 ? cache->k : p.q, p.dtype, d, st, b)) return rc;
+    if (int rc = make_tmap_4d(&tv, cache->pages > 0 ? cache->v : p.q, p.dtype, d, st, b)) return rc;
+  } else {
+    const int64_t rows = p.kv_rows > 0 ? p.kv_rows : 1;   // without keys nothing is copied through the maps
+    const int64_t d[4] = {p.dim, rows, p.kv_heads, 1};
+    const int64_t ks[3] = {p.k_token * 2, p.k_head * 2, p.k_token * 2}, vs[3] = {p.v_token * 2, p.v_head * 2, p.v_token * 2};
+    const int b[4] = {64, box_keys, 1, 1};
+    if (int rc = make_tmap_4d(&tk, p.kv_rows > 0 ? p.k : p.q, p.dtype, d, ks, b)) return rc;
+    if (int rc = make_tmap_4d(&tv, p.kv_rows > 0 ? p.v : p.q, p.dtype, d, vs, b)) return rc;
+  }
+  int* status = nullptr;
+  if (int rc = device_status_word(&status)) return rc;
+  const size_t smem = 1024 + static_cast<size_t>(spans * kSpanBytes) * (2 + (spans == 2 ? 5 : 8)) + 512;
+  const PagedCache none{};
+  auto launch = [&](auto kernel, uint32_t fmt) -> int {
+    FB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    kernel<<<static_cast<unsigned>(grid), kTilesThreads, smem, stream>>>(tq, tk, tv, p, cache != nullptr ? *cache : none, tile_tokens,
+                                                                         box_keys, fmt, status);
+    return FB200_OK;
+  };
+  const bool bf = p.dtype == FB200_BF16;
+  int rc = FB200_OK;
+  if (cache != nullptr) {
+    if (spans == 2) rc = bf ? launch(attention_tiles_kernel<__nv_bfloat16, 2, true>, kFmtBF16) : launch(attention_tiles_kernel<__half, 2, true>, kFmtF16);
+    else rc = bf ? launch(attention_tiles_kernel<__nv_bfloat16, 1, true>, kFmtBF16) : launch(attention_tiles_kernel<__half, 1, true>, kFmtF16);
+  } else {
+    if (spans == 2) rc = bf ? launch(attention_tiles_kernel<__nv_bfloat16, 2, false>, kFmtBF16) : launch(attention_tiles_kernel<__half, 2, false>, kFmtF16);
+    else rc = bf ? launch(attention_tiles_kernel<__nv_bfloat16, 1, false>, kFmtBF16) : launch(attention_tiles_kernel<__half, 1, false>, kFmtF16);
+  }
+  if (rc != FB200_OK) return rc;
+  return after_launch("attention_tiles_kernel");
+}
+
+}  // namespace fb200

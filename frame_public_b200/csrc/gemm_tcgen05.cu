@@ -877,6 +877,28 @@ int make_tmap_nchw_f32(CUtensorMap* map, const void* ptr, int64_t n, int64_t c, 
   return FB200_OK;
 }
 
+// Four dimensions of 16-bit elements (innermost contiguous, the other strides in bytes), boxes 128 bytes
+// wide with the 128-byte swizzle, zero fill outside.
+int make_tmap_4d(CUtensorMap* map, const void* ptr, int dtype, const int64_t (&dims)[4], const int64_t (&stride_bytes)[3],
+                 const int (&box)[4]) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return set_error(FB200_DEVICE_ERROR, "cuTensorMapEncodeTiled is not available");
+  cuuint64_t gdim[4], gstride[3];
+  cuuint32_t gbox[4], estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) {
+    gdim[i] = static_cast<cuuint64_t>(dims[i]);
+    gbox[i] = static_cast<cuuint32_t>(box[i]);
+    if (i < 3) gstride[i] = static_cast<cuuint64_t>(stride_bytes[i]);
+  }
+  CUresult r = fn(map, dtype == FB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                  const_cast<void*>(ptr), gdim, gstride, gbox, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    return set_error(FB200_INTERNAL, "cuTensorMapEncodeTiled (4-D) failed with code %d", static_cast<int>(r));
+  }
+  return FB200_OK;
+}
+
 // Per-device status word the kernels write when a bounded wait gives up (host-mapped, so the
 // host can read it after a stream synchronise without a copy).
 struct StatusWord { int* host = nullptr; int* dev = nullptr; };

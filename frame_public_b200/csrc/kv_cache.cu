@@ -201,7 +201,7 @@ static int check_rows(const char* what, const fb200_kv_cache* cache, const void*
                       int64_t vt, int64_t vh, const int32_t* cu, const int32_t* table, int64_t table_stride,
                       int64_t n_seqs, int64_t rows, int dtype) {
   if (int rc = check_kv_cache(what, cache, dtype)) return rc;
-  if (n_seqs < 0 || n_seqs > INT_MAX - 1 || rows < 0 || rows > INT_MAX || table_stride < 0) {
+  if (n_seqs < 0 || n_seqs > INT_MAX - 1 || rows < 0 || rows > kMostTokens || table_stride < 0) {
     return set_error(FB200_INVALID_ARGUMENT, "%s: bad size (%lld sequences, %lld rows, table stride %lld)", what,
                      (long long)n_seqs, (long long)rows, (long long)table_stride);
   }

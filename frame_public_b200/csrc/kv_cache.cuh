@@ -18,6 +18,8 @@ enum ServingFault : int {
   kFaultBadLength = 322,   // a token outside the block table, or more query rows than max_q
 };
 
+constexpr int64_t kMostTokens = int64_t(1) << 30;   // of a packed tensor or a cached sequence: sums of a few stay in 32 bits
+
 __host__ __device__ inline int64_t clamp_i64(int64_t x, int64_t lo, int64_t hi) {
   return x < lo ? lo : x > hi ? hi : x;
 }
@@ -70,7 +72,7 @@ __device__ __forceinline__ int page_number(const PagedCache& c, int64_t s, int64
 // Cached tokens of a sequence, cut to what its table row can hold.
 __host__ __device__ inline int cached_length(int32_t kv_len, int64_t table_stride, int page_shift) {
   const int64_t most = table_stride << page_shift;
-  return static_cast<int>(clamp_i64(kv_len, 0, most < 0x7fffffff ? most : 0x7fffffff));
+  return static_cast<int>(clamp_i64(kv_len, 0, most < kMostTokens ? most : kMostTokens));
 }
 
 __device__ __forceinline__ int64_t token_offset(const PagedCache& c, int page, int token, int head) {
