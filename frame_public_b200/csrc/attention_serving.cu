@@ -157,7 +157,7 @@ extern "C" int fb200_attention_prompt(const fb200_attention_params* params, cons
   r.k_head = params->k_head_stride;
   r.v_token = params->v_token_stride;
   r.v_head = params->v_head_stride;
-  return launch_attention_tiles(r, nullptr, nullptr, as_stream(stream));
+  return launch_attention_tiles(r, nullptr, as_stream(stream));
 }
 
 static int check_paged(const char* what, const fb200_attention_params* p, const fb200_kv_cache* c) {
@@ -172,7 +172,10 @@ static int check_paged(const char* what, const fb200_attention_params* p, const 
 extern "C" int fb200_attention_paged_workspace(const fb200_attention_params* params, const fb200_kv_cache* cache, size_t* bytes) {
   if (bytes == nullptr) return set_error(FB200_INVALID_ARGUMENT, "attention_paged_workspace: null out pointer");
   *bytes = 0;
-  return check_paged("attention_paged_workspace", params, cache);
+  if (int rc = check_paged("attention_paged_workspace", params, cache)) return rc;
+  const ServingProblem r = make_problem(params, nullptr, nullptr, nullptr, nullptr);
+  if (attention_decode_takes(r)) *bytes = attention_decode_workspace(r);
+  return FB200_OK;
 }
 
 extern "C" int fb200_attention_paged(const fb200_attention_params* params, const fb200_kv_cache* cache, const void* q, void* o,
@@ -195,6 +198,7 @@ extern "C" int fb200_attention_paged(const fb200_attention_params* params, const
   if (int rc = make_paged_cache(cache, block_table, table_stride, &c)) return rc;
   ServingProblem r = make_problem(params, q, o, lse, cu_q);
   r.kv_len = kv_len;
-  if (cache->dtype != FB200_U8 && params->max_q * r.group > 16) return launch_attention_tiles(r, &c, cache, as_stream(stream));
+  if (attention_decode_takes(r)) return launch_attention_decode(r, c, cache->dtype == FB200_U8, workspace, as_stream(stream));
+  if (cache->dtype != FB200_U8) return launch_attention_tiles(r, &c, as_stream(stream));
   return launch_rows(r, c, true, cache->dtype == FB200_U8, params->dtype, as_stream(stream));
 }

@@ -420,7 +420,7 @@ static int64_t most_blocks(const ServingProblem& p, int64_t tokens) {
   return by_rows < by_seq ? by_rows : by_seq;
 }
 
-int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, const fb200_kv_cache* desc, cudaStream_t stream) {
+int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, cudaStream_t stream) {
   const int tile_tokens = kTileRows / p.group;
   const int64_t grid = most_blocks(p, 2 * tile_tokens) * p.kv_heads;
   if (grid > 0x7fffffff) return set_error(FB200_INVALID_ARGUMENT, "attention: too many tiles");
