@@ -145,6 +145,19 @@ __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int 
   return false;
 }
 
+// A place in the ring; K and V tiles alternate, so each steps by two.
+struct RingPos {
+  int slot;
+  uint32_t phase;
+  __device__ __forceinline__ void next(int slots) {
+    slot += 2;
+    if (slot >= slots) {
+      slot -= slots;
+      phase ^= 1u;
+    }
+  }
+};
+
 template <typename T, int SPANS, bool PAGED>
 __global__ void __launch_bounds__(kTilesThreads, 1)
 attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -194,8 +207,11 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   __syncthreads();
   tcgen05_fence_after_sync();
   const uint32_t tmem = *tmem_slot_ptr;
-  const TilesItem item = *item_ptr;
-  const bool work = *found_ptr != 0;
+  // Broadcasts, so that the compiler knows the warp-uniform values that steer the tensor-core warp.
+  auto uniform = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+  const TilesItem item{uniform(item_ptr->seq), uniform(item_ptr->block), uniform(item_ptr->q0),
+                       uniform(item_ptr->lq), uniform(item_ptr->k0), uniform(item_ptr->lk)};
+  const bool work = uniform(*found_ptr) != 0;
   const int token0 = item.block * 2 * tile_tokens;
   int tiles[2];
 #pragma unroll
@@ -234,7 +250,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           page = page_number(cache, item.seq, key >> cache.page_shift, status);
           row = key & ((1 << cache.page_shift) - 1);
         }
-        if (use > 0) live = mbar_wait_warp(freed + 8 * slot, (use - 1) & 1, status, kFaultTilesRing);
+        if (use > 0) live = mbar_wait_lanes(freed + 8 * slot, (use - 1) & 1, status, kFaultTilesRing);
         if (!live) break;
         if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(boxes * box_keys * 128 * SPANS));
         __syncwarp();
@@ -248,6 +264,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     __syncwarp();
   } else if (warp == 8) {
     // ---- products --------------------------------------------------------------------------------
+    // Straight-line issue: descriptors and ring positions advance by additions in warp-uniform code (a
+    // division per tile and a rolled loop over the k steps took 2900 cycles per 128 x 128 x 128 pair of
+    // products, three times what the tensor core needs for it).
     if (most > 0) {
       const int k_steps = p.dim / 16;
       const uint32_t idesc_s = make_instr_desc(fmt, 0, 0, kTileRows, kTileKeys);
@@ -255,53 +274,72 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       const uint64_t q_desc = make_smem_desc_sw128(q_s, 16, 1024);
       const uint64_t k_desc = make_smem_desc_sw128(ring, 16, 1024);
       const uint64_t v_desc = make_smem_desc(ring, kSpanBytes, 1024, kLayoutSw128);
-      bool live = mbar_wait_warp(bar_q, 0, status, kFaultTilesQuery);
-      auto scores = [&](int s, int j) {
-        const int n = 2 * j, slot = n % kSlots;
-        live = live && mbar_wait_warp(full + 8 * slot, (n / kSlots) & 1, status, kFaultTilesKeys);
-        if (!live) return;
+      bool live = mbar_wait_lanes(bar_q, 0, status, kFaultTilesQuery);
+      RingPos kp{0, 0}, vp{1, 0};   // of the K and the V tile that come next
+      auto keys_there = [&] {
+        live = live && mbar_wait_lanes(full + 8 * kp.slot, kp.phase, status, kFaultTilesKeys);
         tcgen05_fence_after_sync();
-        const uint64_t a = q_desc + static_cast<uint64_t>(s * kSlotBytes / 16), b = k_desc + static_cast<uint64_t>(slot * kSlotBytes / 16);
-        for (int k = 0; k < k_steps; ++k) {
-          const uint64_t at = static_cast<uint64_t>((k >> 2) * (kSpanBytes / 16) + (k & 3) * 2);
-          mma_f16_elect(tmem + s * kTileKeys, a + at, b + at, idesc_s, k > 0 ? 1u : 0u);
+      };
+      auto scores = [&](int s) {
+        const uint64_t a = q_desc + static_cast<uint64_t>(s * (kSlotBytes / 16)), b = k_desc + static_cast<uint64_t>(kp.slot * (kSlotBytes / 16));
+        constexpr uint64_t kSpanUnits = kSpanBytes / 16;
+#pragma unroll
+        for (int x = 0; x < SPANS; ++x) {
+          if (k_steps >= x * 4 + 4) {
+            mma_f16_elect_x4<2, 2>(tmem + s * kTileKeys, a + x * kSpanUnits, b + x * kSpanUnits, idesc_s, x > 0 ? 1u : 0u);
+          } else {   // a head_dim that is no multiple of 64 ends inside a span
+            for (int k = x * 4; k < k_steps; ++k) {
+              const uint64_t at = x * kSpanUnits + (k & 3) * 2;
+              mma_f16_elect(tmem + s * kTileKeys, a + at, b + at, idesc_s, k > 0 ? 1u : 0u);
+            }
+          }
         }
         mma_commit_elect(bar_s + 8 * s);
-        if (s == 1 || j >= tiles[1]) mma_commit_elect(freed + 8 * slot);   // the last reader
       };
       auto values = [&](int s, int j) {
-        const int n = 2 * j + 1, slot = n % kSlots;
-        live = live && mbar_wait_warp(full + 8 * slot, (n / kSlots) & 1, status, kFaultTilesKeys);
-        live = live && mbar_wait_warp(bar_p + 8 * s, j & 1, status, kFaultTilesProbs);
+        live = live && mbar_wait_lanes(bar_p + 8 * s, j & 1, status, kFaultTilesProbs);
         if (!live) return;
+        tcgen05_fence_after_sync();
+        const uint64_t b = v_desc + static_cast<uint64_t>(vp.slot * (kSlotBytes / 16));
+#pragma unroll
+        for (int k = 0; k < kTileKeys / 16; k += 4) {
+          mma_f16_ts_elect_x4<8, 128>(tmem + kTmemO + s * (SPANS * 64), tmem + s * kTileKeys + k * 8, b + k * 128, idesc_o,
+                                      (j > 0 || k > 0) ? 1u : 0u);
+        }
+        if (j + 1 == tiles[s]) mma_commit_elect(bar_o + 8 * s);
+      };
+      keys_there();
+      if (live && tiles[0] > 0) scores(0);
+      if (live && tiles[1] > 0) scores(1);
+      mma_commit_elect(freed + 8 * kp.slot);
+      kp.next(kSlots);
+      for (int j = 0; live && j < most; ++j) {
+        live = mbar_wait_lanes(full + 8 * vp.slot, vp.phase, status, kFaultTilesKeys);
+        if (!live) break;
         const int there = item.lk - j * kTileKeys;
-        if (there < kTileKeys && (s == 0 || j >= tiles[0])) {
+        if (there < kTileKeys) {
           // Rows behind the last key hold another sequence's values or none: their P is 0, but 0 times a
           // NaN is not.
           for (int i = lane; i < (kTileKeys - there) * 8 * SPANS; i += 32) {
             const int row = there + (i >> 3) % (kTileKeys - there), span = (i >> 3) / (kTileKeys - there);
-            *reinterpret_cast<uint4*>(base_ptr + (ring - base) + slot * kSlotBytes + span * kSpanBytes + row * 128 + (i & 7) * 16) =
+            *reinterpret_cast<uint4*>(base_ptr + (ring - base) + vp.slot * kSlotBytes + span * kSpanBytes + row * 128 + (i & 7) * 16) =
                 make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
           __syncwarp();
         }
-        tcgen05_fence_after_sync();
-        const uint64_t b = v_desc + static_cast<uint64_t>(slot * kSlotBytes / 16);
-#pragma unroll
-        for (int k = 0; k < kTileKeys / 16; ++k) {
-          mma_f16_ts_elect(tmem + kTmemO + s * (SPANS * 64), tmem + s * kTileKeys + k * 8, b + k * 128, idesc_o, (j > 0 || k > 0) ? 1u : 0u);
-        }
-        if (s == 1 || j >= tiles[1]) mma_commit_elect(freed + 8 * slot);
-        if (j + 1 == tiles[s]) mma_commit_elect(bar_o + 8 * s);
-      };
-      for (int s = 0; s < 2; ++s) {
-        if (tiles[s] > 0) scores(s, 0);
-      }
-      for (int j = 0; live && j < most; ++j) {
-        for (int s = 0; s < 2; ++s) {
-          if (j < tiles[s]) values(s, j);
-          if (j + 1 < tiles[s]) scores(s, j + 1);
+        const bool more = j + 1 < most;
+        if (j < tiles[0]) values(0, j);
+        if (more) keys_there();
+        if (live && j + 1 < tiles[0]) scores(0);
+        if (live && j < tiles[1]) values(1, j);
+        if (!live) break;
+        mma_commit_elect(freed + 8 * vp.slot);
+        vp.next(kSlots);
+        if (more) {
+          if (j + 1 < tiles[1]) scores(1);
+          mma_commit_elect(freed + 8 * kp.slot);
+          kp.next(kSlots);
         }
       }
     }
@@ -319,7 +357,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     float m = -INFINITY, l = 0.0f;
     bool live = true;
     for (int j = 0; j < tiles[s]; ++j) {
-      live = mbar_wait_warp(bar_s + 8 * s, j & 1, status, kFaultTilesScores);
+      live = mbar_wait_lanes(bar_s + 8 * s, j & 1, status, kFaultTilesScores);
       if (!live) break;
       tcgen05_fence_after_sync();
       uint32_t r[4][32];
@@ -379,7 +417,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       if (lane == 0) mbar_arrive(bar_p + 8 * s);
     }
     const bool any = tiles[s] > 0;
-    if (any && live) live = mbar_wait_warp(bar_o + 8 * s, 0, status, kFaultTilesOutput);
+    if (any && live) live = mbar_wait_lanes(bar_o + 8 * s, 0, status, kFaultTilesOutput);
     if (live) {
       tcgen05_fence_after_sync();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;

@@ -83,6 +83,16 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, in
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
+// The same wait with every lane polling: no branch around the poll and no broadcast behind it, which
+// makes a wait that is already over several times cheaper for a warp that issues tensor instructions.
+__device__ __forceinline__ bool mbar_wait_lanes(uint32_t bar, uint32_t parity, int* status, int code) {
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  }
+  return mbar_wait_warp(bar, parity, status, code);
+}
+
 // ---- proxies and fences -----------------------------------------------------------------------
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -304,18 +314,59 @@ __device__ __forceinline__ void mma_f16_elect(uint32_t d_tmem, uint64_t a_desc, 
       : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// A from tensor memory: row i of A lies in lane i, two 16-bit elements per column (the lower k first).
-__device__ __forceinline__ void mma_f16_ts_elect(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+// Four consecutive K steps in one block: one election, descriptors advanced inside it (`step` in units of
+// 16 bytes).  The accumulate flag is the first step's; the others add.
+template <int A_STEP, int B_STEP>
+__device__ __forceinline__ void mma_f16_elect_x4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                                  uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
-      ".reg .pred p, q;\n\t"
+      ".reg .pred p, q, t;\n\t"
+      ".reg .b64 a, b;\n\t"
       "elect.sync _|q, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "add.s64 a, %1, %5;\n\t"
+      "add.s64 b, %2, %6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+      "add.s64 a, a, %5;\n\t"
+      "add.s64 b, b, %6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+      "add.s64 a, a, %5;\n\t"
+      "add.s64 b, b, %6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
       "}\n"
       :
-      : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "n"(A_STEP), "n"(B_STEP)
+      : "memory");
+}
+// The same with A in tensor memory: row i of A lies in lane i, two 16-bit elements per column (the lower
+// k first), A_STEP in columns.
+template <int A_STEP, int B_STEP>
+__device__ __forceinline__ void mma_f16_ts_elect_x4(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                                    uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q, t;\n\t"
+      ".reg .b64 b;\n\t"
+      ".reg .b32 a;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "add.s32 a, %1, %5;\n\t"
+      "add.s64 b, %2, %6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+      "add.s32 a, a, %5;\n\t"
+      "add.s64 b, b, %6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+      "add.s32 a, a, %5;\n\t"
+      "add.s64 b, b, %6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+      "}\n"
+      :
+      : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "n"(A_STEP), "n"(B_STEP)
       : "memory");
 }
 __device__ __forceinline__ void mma_tf32_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
