@@ -8,18 +8,25 @@
 // chunks of new tokens still fill the tensor core's 128 rows.
 //
 // A CTA holds two such tiles ("stages") and walks the keys both see.  Roles:
-//   warps 0-3, 4-7   softmax of stage 0 and 1, one thread per row = TMEM lane: tcgen05.ld of the row's
-//                    128 scores, maximum, exponentials, tcgen05.st of P (16 bit) over S
-//   warp 8           every tcgen05.mma: S_s = Q_s K^T (both operands in shared memory), O_s += P_s V with
+//   warps 0-7, 8-15  softmax of stage 0 and 1, two threads per row = TMEM lane with 64 keys each:
+//                    tcgen05.ld of the scores, maximum, exponentials, tcgen05.st of P (16 bit); a quarter of
+//                    the exponentials is a polynomial on the FMA pipe instead of ex2 on the XU pipe
+//   warp 16          every tcgen05.mma: S_s = Q_s K^T (both operands in shared memory), O_s += P_s V with
 //                    P as the A operand in TMEM, so P never passes through shared memory
-//   warp 9           TMA: Q once, K and V tiles through a ring; a paged cache one box per page
-// While the threads of one stage compute exponentials the tensor core works on the other one.  TMEM:
-// S0, S1 (128 columns each, P over the first 64), O0, O1.
+//   warp 17          TMA: Q once, K and V tiles through a ring; a paged cache one box per page
+// While the threads of one stage compute exponentials the tensor core works for the other one.  TMEM has
+// 512 columns.  head_dim up to 64: S0, S1 (128 each), O0, O1, P0, P1 (64 each), and the scores of the next
+// tile are computed as soon as the threads have read those of this one.  Above: S0, S1, O0, O1 (128 each)
+// leave no room, P lies over S, and the next scores follow P V; P is handed over in halves so that only
+// the second half of P V lies between the two.
 // O is only rescaled when a row's maximum grew by more than 2^8 since the last time (the exponents stay
 // below 2^8 then, which fp32 sums and 16-bit P hold as well as values up to 1).
 //
 // Bounds: 4 * pairs * head_dim FLOP against the tensor pipe; one exponential per pair against the
 // XU pipe (16 per SM and cycle: 1024 cycles for a 128 x 128 tile whose two products take 512 to 1024).
+// Shared memory is next: a score instruction of N columns reads (128 + N) * 32 bytes at 128 bytes per cycle,
+// which for N = 64 is 48 cycles against 32 in the tensor pipe (measured), for N = 128 the 64 of both.  So
+// scores are computed 128 keys at a time (steps of 64 took 584 us where these take 518, 2x8192 d128).
 #include <cuda.h>
 
 #include "attention_serving.cuh"
@@ -35,7 +42,10 @@ using namespace sm100;
 
 constexpr int kTileRows = 128;
 constexpr int kTileKeys = 128;
-constexpr int kTilesThreads = 320;
+constexpr int kSoftmaxWarps = 16;             // two threads per row of each stage, 64 of the 128 keys each
+constexpr int kMmaWarp = kSoftmaxWarps, kCopyWarp = kSoftmaxWarps + 1;
+constexpr int kTilesThreads = (kSoftmaxWarps + 2) * 32;
+constexpr int kHalfKeys = kTileKeys / 2;
 constexpr int kSpanBytes = kTileRows * 128;   // 128 rows of 64 16-bit elements
 constexpr float kRescaleStep = 8.0f;          // log2 of the growth of a row's maximum that O follows at once
 
@@ -52,6 +62,26 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 2^x without the XU pipe: x = n + f with f in [-1/2, 1/2] by adding 1.5 * 2^23 (n stands in the low bits of
+// the sum), 2^f by the polynomial of degree 5 with the least largest relative error (1.6e-7 in fp32
+// arithmetic; found by reweighted least squares, constant term 1), n added to its exponent.  From -127 down:
+// f = 0 and the exponent field becomes 0, which is exactly 0.  A NaN stays in the maximum and ends as the
+// largest number, which becomes an infinity in P and NaN in O.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));   // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
+  const float2 big = make_float2(12582912.0f, 12582912.0f), t = __fadd2_rn(x, big);
+  const float2 n = __fadd2_rn(t, make_float2(-12582912.0f, -12582912.0f));
+  const float2 f = __fadd2_rn(x, make_float2(-n.x, -n.y));
+  auto both = [](float a) { return make_float2(a, a); };
+  float2 y = __ffma2_rn(both(0.0013264727f), f, both(0.009671513f));
+  y = __ffma2_rn(y, f, both(0.055507336f));
+  y = __ffma2_rn(y, f, both(0.24022242f));
+  y = __ffma2_rn(y, f, both(0.693147f));
+  y = __ffma2_rn(y, f, both(1.0f));
+  return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
 }
 template <typename T> __device__ __forceinline__ uint32_t pack_pair(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float lo, float hi) {
@@ -145,6 +175,9 @@ __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int 
   return false;
 }
 
+// Barriers and the swap of row maxima, in front of the tiles.
+__host__ __device__ constexpr uint32_t kTilesSmallBytes(int spans) { return 320 + (spans == 1 ? 2 : 1) * 4 * kTileRows * 4; }
+
 // A place in the ring; K and V tiles alternate, so each steps by two.
 struct RingPos {
   int slot;
@@ -165,18 +198,19 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                        int tile_tokens, int box_keys, uint32_t fmt, int* status) {
   constexpr int kSlotBytes = SPANS * kSpanBytes;
   constexpr int kSlots = SPANS == 2 ? 5 : 8;
-  constexpr uint32_t kTmemO = 2 * kTileKeys;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw_addr = smem_u32(smem_raw);
-  const uint32_t base = (raw_addr + 1023u) & ~1023u;
-  uint8_t* base_ptr = smem_raw + (base - raw_addr);
-  const uint32_t q_s = base, ring = base + 2 * kSlotBytes, bars = ring + kSlots * kSlotBytes;
-  const uint32_t bar_q = bars, full = bars + 8, freed = full + 8 * kSlots, bar_s = freed + 8 * kSlots, bar_p = bar_s + 16,
-                 bar_o = bar_p + 16, tmem_slot = bar_o + 16;
-  uint8_t* const after = base_ptr + (tmem_slot - base);
+  constexpr bool kApart = SPANS == 1;   // P has columns of its own
+  constexpr uint32_t kTmemO = 2 * kTileKeys, kTmemP = kApart ? kTmemO + 128 : 0, kTmemPStage = kApart ? 64 : kTileKeys;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t bars = smem_u32(smem_raw), base = (bars + kTilesSmallBytes(SPANS) + 1023u) & ~1023u;   // swizzle atoms are 1024 bytes
+  uint8_t* base_ptr = smem_raw + (base - bars);
+  const uint32_t q_s = base, ring = base + 2 * kSlotBytes;
+  const uint32_t bar_q = bars, full = bars + 8, freed = full + 8 * kSlots, bar_s = freed + 8 * kSlots, bar_r = bar_s + 16,
+                 bar_p = bar_r + 16, bar_o = bar_p + 32, tmem_slot = bar_o + 16;
+  uint8_t* const after = smem_raw + (tmem_slot - bars);
   volatile uint32_t* const tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(after);
   TilesItem* const item_ptr = reinterpret_cast<TilesItem*>(after + 16);
   int* const found_ptr = reinterpret_cast<int*>(after + 16 + sizeof(TilesItem));
+  float* const share = reinterpret_cast<float*>(smem_raw + 320);   // [tile parity, P apart only][stage][half][row]: maxima, then sums
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.x % p.kv_heads;
@@ -187,7 +221,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       if (found) *item_ptr = it;
       *found_ptr = found;
     }
-  } else if (warp == 8 && lane == 0) {
+  } else if (warp == kMmaWarp && lane == 0) {
     mbar_init(bar_q, 1);
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(full + 8 * i, 1);
@@ -195,20 +229,23 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_s + 8 * i, 1);
-      mbar_init(bar_p + 8 * i, 4);
+      mbar_init(bar_r + 8 * i, kSoftmaxWarps / 2);
+      mbar_init(bar_p + 16 * i, 4);
+      mbar_init(bar_p + 16 * i + 8, 4);
       mbar_init(bar_o + 8 * i, 1);
     }
     mbar_fence_init();
-  } else if (warp == 9) {
+  } else if (warp == kCopyWarp) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   tcgen05_fence_before_sync();
   __syncthreads();
   tcgen05_fence_after_sync();
-  const uint32_t tmem = *tmem_slot_ptr;
-  // Broadcasts, so that the compiler knows the warp-uniform values that steer the tensor-core warp.
-  auto uniform = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+  // Equal in all lanes; a warp reduction leaves its result in a uniform register, which is where the
+  // descriptors, addresses and loop bounds of the tensor instructions have to be.
+  auto uniform = [](int x) { return __reduce_max_sync(0xffffffffu, x); };
+  const uint32_t tmem = __reduce_max_sync(0xffffffffu, *tmem_slot_ptr);
   const TilesItem item{uniform(item_ptr->seq), uniform(item_ptr->block), uniform(item_ptr->q0),
                        uniform(item_ptr->lq), uniform(item_ptr->k0), uniform(item_ptr->lk)};
   const bool work = uniform(*found_ptr) != 0;
@@ -221,9 +258,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                    ? (keys_seen(p.causal, min(item.lq, first + tile_tokens), item.lq, item.lk) + kTileKeys - 1) / kTileKeys
                    : 0;
   }
-  const int most = max(tiles[0], tiles[1]);   // stage 1's rows come later: it sees as many, unless it has none
+  const int most = max(tiles[0], tiles[1]);   // stage 1's rows come later: it sees as much, unless it has none
 
-  if (warp == 9) {
+  if (warp == kCopyWarp) {
     // ---- copies ----------------------------------------------------------------------------------
     if (most > 0) {
       if (lane == 0) {
@@ -262,7 +299,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
     }
     __syncwarp();
-  } else if (warp == 8) {
+  } else if (warp == kMmaWarp) {
     // ---- products --------------------------------------------------------------------------------
     // Straight-line issue: descriptors and ring positions advance by additions in warp-uniform code (a
     // division per tile and a rolled loop over the k steps took 2900 cycles per 128 x 128 x 128 pair of
@@ -276,45 +313,56 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       const uint64_t v_desc = make_smem_desc(ring, kSpanBytes, 1024, kLayoutSw128);
       bool live = mbar_wait_lanes(bar_q, 0, status, kFaultTilesQuery);
       RingPos kp{0, 0}, vp{1, 0};   // of the K and the V tile that come next
-      auto keys_there = [&] {
-        live = live && mbar_wait_lanes(full + 8 * kp.slot, kp.phase, status, kFaultTilesKeys);
-        tcgen05_fence_after_sync();
-      };
       auto scores = [&](int s) {
         const uint64_t a = q_desc + static_cast<uint64_t>(s * (kSlotBytes / 16)), b = k_desc + static_cast<uint64_t>(kp.slot * (kSlotBytes / 16));
+        const uint32_t d = tmem + s * kTileKeys;
         constexpr uint64_t kSpanUnits = kSpanBytes / 16;
 #pragma unroll
         for (int x = 0; x < SPANS; ++x) {
           if (k_steps >= x * 4 + 4) {
-            mma_f16_elect_x4<2, 2>(tmem + s * kTileKeys, a + x * kSpanUnits, b + x * kSpanUnits, idesc_s, x > 0 ? 1u : 0u);
+            mma_f16_elect_x4<2, 2>(d, a + x * kSpanUnits, b + x * kSpanUnits, idesc_s, x > 0 ? 1u : 0u);
           } else {   // a head_dim that is no multiple of 64 ends inside a span
             for (int k = x * 4; k < k_steps; ++k) {
               const uint64_t at = x * kSpanUnits + (k & 3) * 2;
-              mma_f16_elect(tmem + s * kTileKeys, a + at, b + at, idesc_s, k > 0 ? 1u : 0u);
+              mma_f16_elect(d, a + at, b + at, idesc_s, k > 0 ? 1u : 0u);
             }
           }
         }
         mma_commit_elect(bar_s + 8 * s);
       };
       auto values = [&](int s, int j) {
-        live = live && mbar_wait_lanes(bar_p + 8 * s, j & 1, status, kFaultTilesProbs);
-        if (!live) return;
-        tcgen05_fence_after_sync();
         const uint64_t b = v_desc + static_cast<uint64_t>(vp.slot * (kSlotBytes / 16));
+        const uint32_t d = tmem + kTmemO + s * (SPANS * 64), a = tmem + kTmemP + s * kTmemPStage;
 #pragma unroll
-        for (int k = 0; k < kTileKeys / 16; k += 4) {
-          mma_f16_ts_elect_x4<8, 128>(tmem + kTmemO + s * (SPANS * 64), tmem + s * kTileKeys + k * 8, b + k * 128, idesc_o,
-                                      (j > 0 || k > 0) ? 1u : 0u);
+        for (int half = 0; half < 2; ++half) {
+          live = live && mbar_wait_lanes(bar_p + 16 * s + 8 * half, j & 1, status, kFaultTilesProbs);
+          if (!live) return;
+          tcgen05_fence_after_sync();
+          mma_f16_ts_elect_x4<8, 128>(d, a + half * 32, b + half * 512, idesc_o, (j > 0 || half > 0) ? 1u : 0u);
         }
-        if (j + 1 == tiles[s]) mma_commit_elect(bar_o + 8 * s);
+        mma_commit_elect(bar_o + 8 * s);
       };
-      keys_there();
-      if (live && tiles[0] > 0) scores(0);
-      if (live && tiles[1] > 0) scores(1);
-      mma_commit_elect(freed + 8 * kp.slot);
-      kp.next(kSlots);
+      live = live && mbar_wait_lanes(full, 0, status, kFaultTilesKeys);
+      tcgen05_fence_after_sync();
+      if (live) {
+        if (tiles[0] > 0) scores(0);
+        if (tiles[1] > 0) scores(1);
+        mma_commit_elect(freed);
+        kp.next(kSlots);
+      }
       for (int j = 0; live && j < most; ++j) {
-        live = mbar_wait_lanes(full + 8 * vp.slot, vp.phase, status, kFaultTilesKeys);
+        const bool more = j + 1 < most;
+        if (more) live = mbar_wait_lanes(full + 8 * kp.slot, kp.phase, status, kFaultTilesKeys);
+        if (kApart && more && live) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if (j + 1 >= tiles[s]) continue;
+            live = live && mbar_wait_lanes(bar_r + 8 * s, j & 1, status, kFaultTilesScores);
+            tcgen05_fence_after_sync();
+            if (live) scores(s);
+          }
+        }
+        live = live && mbar_wait_lanes(full + 8 * vp.slot, vp.phase, status, kFaultTilesKeys);
         if (!live) break;
         const int there = item.lk - j * kTileKeys;
         if (there < kTileKeys) {
@@ -328,16 +376,15 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           fence_proxy_async_smem();
           __syncwarp();
         }
-        const bool more = j + 1 < most;
-        if (j < tiles[0]) values(0, j);
-        if (more) keys_there();
-        if (live && j + 1 < tiles[0]) scores(0);
-        if (live && j < tiles[1]) values(1, j);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (live && j < tiles[s]) values(s, j);
+          if (!kApart && live && j + 1 < tiles[s]) scores(s);
+        }
         if (!live) break;
         mma_commit_elect(freed + 8 * vp.slot);
         vp.next(kSlots);
         if (more) {
-          if (j + 1 < tiles[1]) scores(1);
           mma_commit_elect(freed + 8 * kp.slot);
           kp.next(kSlots);
         }
@@ -346,47 +393,78 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     __syncwarp();
   } else {
     // ---- softmax ---------------------------------------------------------------------------------
-    const int s = warp >> 2, row = threadIdx.x & 127;
+    const int s = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & 127;
     const int in_tile = row / p.group, token = token0 + s * tile_tokens + in_tile;
     const int h = head * p.group + row - in_tile * p.group;
     const bool there = work && in_tile < tile_tokens && token < item.lq;
     const int limit = there ? keys_seen(p.causal, token + 1, item.lq, item.lk) : 0;   // keys this row sees
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t t_s = lanes + s * kTileKeys, t_o = lanes + kTmemO + s * (SPANS * 64);
+    const uint32_t t_s = lanes + s * kTileKeys + half * kHalfKeys, t_p = lanes + kTmemP + s * kTmemPStage + half * (kHalfKeys / 2);
+    const uint32_t t_o = lanes + kTmemO + s * (SPANS * 64);
+    float* const mine = share + (s * 2 + half) * kTileRows + row;
+    const float* const other = share + (s * 2 + 1 - half) * kTileRows + row;
+    // The two warps that hold the halves of the same 32 rows meet; true if both are still live, so that they
+    // give up at the same tile.
+    auto pair_sync = [&](bool ok) {
+      uint32_t all;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbar.red.and.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+                   : "=r"(all) : "r"(1 + s * 4 + (warp & 3)), "r"(ok ? 1u : 0u) : "memory");
+      return all != 0;
+    };
     const float c = p.scale * 1.4426950408889634f;
     float m = -INFINITY, l = 0.0f;
     bool live = true;
     for (int j = 0; j < tiles[s]; ++j) {
       live = mbar_wait_lanes(bar_s + 8 * s, j & 1, status, kFaultTilesScores);
-      if (!live) break;
       tcgen05_fence_after_sync();
-      uint32_t r[4][32];
+      uint32_t r[2][32];
+      tmem_ld_32x32b_x32(t_s, r[0]);
+      tmem_ld_32x32b_x32(t_s + 32, r[1]);
+      tmem_ld_wait(r[0]);
+      tmem_ld_wait(r[1]);
+      if constexpr (kApart) {   // the next tile's scores may come
+        tcgen05_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_r + 8 * s);
+      }
+      const int visible = limit - j * kTileKeys - half * kHalfKeys;
+      if (__any_sync(0xffffffffu, visible < kHalfKeys)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_s + i * 32, r[i]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld_wait(r[i]);
-      const int visible = limit - j * kTileKeys;
-      if (__any_sync(0xffffffffu, visible < kTileKeys)) {
-#pragma unroll
-        for (int i = 0; i < 128; ++i) {
+        for (int i = 0; i < kHalfKeys; ++i) {
           if (i >= visible) r[i >> 5][i & 31] = 0xFF800000u;   // -inf
         }
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 128; i += 2) {
+      for (int i = 0; i < kHalfKeys; i += 2) {
         top[(i >> 1) & 3] = fmaxf(top[(i >> 1) & 3], fmaxf(__uint_as_float(r[i >> 5][i & 31]), __uint_as_float(r[i >> 5][(i & 31) + 1])));
       }
-      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      // P apart: the product of the tile before is done, so P's columns and O are free.  (P over S: the scores
+      // of this tile were issued behind it.)
+      if (kApart && j > 0) {
+        live = mbar_wait_lanes(bar_o + 8 * s, (j - 1) & 1, status, kFaultTilesOutput) && live;
+        tcgen05_fence_after_sync();
+      }
+      // The row's maximum: the halves swap theirs.  With P over S this also keeps one half's P from reaching
+      // columns that the other has not read.  (A place of the swap is written again two tiles on, or, with P
+      // over S, behind the next scores, which wait for both halves' P.)
+      const int swap = kApart ? (j & 1) * 4 * kTileRows : 0;
+      mine[swap] = mx;
+      if constexpr (!kApart) tcgen05_fence_before_sync();
+      live = pair_sync(live);
+      if (!live) break;
+      if constexpr (!kApart) tcgen05_fence_after_sync();
+      mx = fmaxf(mx, other[swap]);
       if (j == 0) {
         m = mx;
       } else if (__any_sync(0xffffffffu, (mx - m) * c > kRescaleStep)) {   // -inf - -inf compares false
-        // The scores of this tile are there, so the products of the previous ones into O are done too.
         const float next = fmaxf(m, mx);
         const float f = next == -INFINITY ? 1.0f : ex2((m - next) * c);
         m = next;
         l *= f;
-        for (int i = 0; i < p.dim; i += 16) {
+        // the first half's threads do it, whose P the tensor core waits for before anything else
+        for (int i = 0; half == 0 && i < p.dim; i += 16) {
           uint32_t x[16];
           tmem_ld_32x32b_x16(t_o + i, x);
           tmem_ld_wait(x);
@@ -399,30 +477,40 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       float2 sum = make_float2(0.0f, 0.0f);
       const float2 c2 = make_float2(c, c), nm2 = make_float2(-mc, -mc);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 2; ++i) {
         uint32_t out[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[i][e]), __uint_as_float(r[i][e + 1])), c2, nm2);
-          const float e0 = ex2(x.x), e1 = ex2(x.y);
-          sum = __fadd2_rn(sum, make_float2(e0, e1));
-          out[e >> 1] = pack_pair<T>(e0, e1);
+          float2 x = __ffma2_rn(make_float2(__uint_as_float(r[i][e]), __uint_as_float(r[i][e + 1])), c2, nm2);
+          if ((e & 7) == 6) {
+            x = exp2_poly(x);
+          } else {
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
+          }
+          sum = __fadd2_rn(sum, x);
+          out[e >> 1] = pack_pair<T>(x.x, x.y);
         }
-        tmem_st_32x32b_x16(t_s + i * 16, out);
+        tmem_st_32x32b_x16(t_p + i * 16, out);
       }
       l += sum.x + sum.y;
       tmem_st_wait();
       tcgen05_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_p + 8 * s);
+      if (lane == 0) mbar_arrive(bar_p + 16 * s + 8 * half);
     }
     const bool any = tiles[s] > 0;
-    if (any && live) live = mbar_wait_lanes(bar_o + 8 * s, 0, status, kFaultTilesOutput);
+    // (The wait before this one's phase is past: above, or by the scores of the last tile.)
+    if (live && any) live = mbar_wait_lanes(bar_o + 8 * s, (tiles[s] - 1) & 1, status, kFaultTilesOutput);
+    live = pair_sync(live);   // the last swap has been read
+    *mine = l;
+    live = pair_sync(live);
+    l += *other;
     if (live) {
       tcgen05_fence_after_sync();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       T* const dst = reinterpret_cast<T*>(p.o) + static_cast<int64_t>(item.q0 + token) * p.o_token + h * p.o_head;
-      for (int i = 0; i < p.dim; i += 16) {
+      for (int i = half * 16; i < p.dim; i += 32) {
         uint32_t x[16];
         if (any) {
           tmem_ld_32x32b_x16(t_o + i, x);
@@ -438,14 +526,14 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           *reinterpret_cast<uint4*>(dst + i + 8) = make_uint4(out[4], out[5], out[6], out[7]);
         }
       }
-      if (there && p.lse != nullptr) {
+      if (there && half == 0 && p.lse != nullptr) {
         p.lse[static_cast<int64_t>(item.q0 + token) * p.heads + h] = l == 0.0f ? -INFINITY : m * p.scale + logf(l);
       }
     }
   }
   tcgen05_fence_before_sync();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kCopyWarp) {
     __syncwarp();
     tmem_dealloc(tmem, 512);
   }
@@ -487,7 +575,7 @@ int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, cud
   }
   int* status = nullptr;
   if (int rc = device_status_word(&status)) return rc;
-  const size_t smem = 1024 + static_cast<size_t>(spans * kSpanBytes) * (2 + (spans == 2 ? 5 : 8)) + 512;
+  const size_t smem = ((kTilesSmallBytes(spans) + 1023) & ~1023u) + static_cast<size_t>(spans * kSpanBytes) * (2 + (spans == 2 ? 5 : 8));
   const PagedCache none{};
   auto launch = [&](auto kernel, uint32_t fmt) -> int {
     FB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
