@@ -111,23 +111,6 @@ __device__ __forceinline__ void cursor_next(const ServingProblem& p, const Paged
   at.left -= at.end;
 }
 
-// ---- e4m3 codes to operands ------------------------------------------------------------------------
-// Codes in the high bytes of the two halves of x (the low bytes are ignored) as a pair of T.  bfloat16:
-// sign, exponent and mantissa move to their places, which is the value times 2^-120 (exponent bias 7
-// against 127; e4m3 denormals become bfloat16 denormals), and one exact product brings it back.  The code
-// 0x7F (NaN) is never written; it reads as 480 here.
-template <typename T> __device__ __forceinline__ uint32_t codes_to_pair(uint32_t x);
-template <> __device__ __forceinline__ uint32_t codes_to_pair<__nv_bfloat16>(uint32_t x) {
-  const uint32_t y = (x & 0x80008000u) | ((x & 0x7F007F00u) >> 4);
-  const uint32_t up = 0x7B807B80u;   // 2^120
-  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&up));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-template <> __device__ __forceinline__ uint32_t codes_to_pair<__half>(uint32_t x) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(__byte_perm(x, 0, 0x4431)), __NV_E4M3);
-  return static_cast<uint32_t>(r.x) | (static_cast<uint32_t>(r.y) << 16);
-}
-
 // BIG: head_dim 65..128, else up to 64.
 template <typename T, bool BIG, bool E4M3>
 __global__ void __launch_bounds__(kDecodeWarps * 32, kDecodeCtasPerSm)

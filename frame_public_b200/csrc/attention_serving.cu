@@ -1,11 +1,9 @@
-// Attention of packed sequences over dense or paged keys and values: one warp per (query row, head).
+// Entry points of attention over packed sequences: checks, and the choice between the two kernels.
 #include "attention_serving.cuh"
 
 #include <climits>
 
 namespace fb200 {
-
-int device_status_word(int** dev_ptr);
 
 int check_attention_params(const char* what, const fb200_attention_params* p) {
   if (p == nullptr) return set_error(FB200_INVALID_ARGUMENT, "%s: null params", what);
@@ -37,65 +35,6 @@ int check_attention_params(const char* what, const fb200_attention_params* p) {
   return FB200_OK;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) attention_rows_kernel(ServingProblem p, PagedCache c, bool paged, bool e4m3, int* status) {
-  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (unit >= static_cast<int64_t>(p.q_rows) * p.heads) return;
-  const int row = static_cast<int>(unit / p.heads), h = static_cast<int>(unit % p.heads), hk = h / p.group;
-  const int s = sequence_of_row(p.cu_q, p.n_seqs, row);
-  if (s < 0) return;
-  int q0, lq, k0 = 0, lk;
-  sequence_span(p.cu_q, s, p.q_rows, q0, lq);
-  if (paged) lk = cached_length(p.kv_len[s], c.table_stride, c.page_shift);
-  else sequence_span(p.cu_kv, s, p.kv_rows, k0, lk);
-  const int last = p.causal ? min(lk - 1, row - q0 + lk - lq) : lk - 1;
-  float q[4], acc[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
-  const T* qp = reinterpret_cast<const T*>(p.q) + row * p.q_token + h * p.q_head;
-  for (int i = 0; i < 4; ++i) q[i] = lane + 32 * i < p.dim ? to_f32(qp[lane + 32 * i]) : 0.0f;
-  for (int j = 0; j <= last; ++j) {
-    float ks = 1.0f, vs = 1.0f;
-    int64_t ka, va;
-    const uint8_t *kb = p.k, *vb = p.v;
-    if (paged) {
-      const int page = page_number(c, s, j >> c.page_shift, status);
-      ka = va = token_offset(c, page, j, hk);
-      kb = c.k;
-      vb = c.v;
-      if (e4m3) {
-        const int64_t at = scale_offset(c, page, j, hk);
-        ks = scale_of_byte(c.k_scale[at]);
-        vs = scale_of_byte(c.v_scale[at]);
-      }
-    } else {
-      ka = (k0 + j) * p.k_token + hk * p.k_head;
-      va = (k0 + j) * p.v_token + hk * p.v_head;
-    }
-    float dot = 0.0f, v[4];
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 32 * i;
-      float kx = 0.0f;
-      v[i] = 0.0f;
-      if (d < p.dim) {
-        kx = e4m3 ? e4m3x2_to_f32(kb[ka + d]).x : to_f32(reinterpret_cast<const T*>(kb)[ka + d]);
-        v[i] = (e4m3 ? e4m3x2_to_f32(vb[va + d]).x : to_f32(reinterpret_cast<const T*>(vb)[va + d])) * vs;
-      }
-      dot += q[i] * kx;
-    }
-    for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-    const float sc = dot * ks * p.scale, nm = fmaxf(m, sc);
-    const float corr = m == -INFINITY ? 0.0f : expf(m - nm), e = nm == -INFINITY ? 0.0f : expf(sc - nm);
-    m = nm;
-    l = l * corr + e;
-    for (int i = 0; i < 4; ++i) acc[i] = acc[i] * corr + e * v[i];
-  }
-  T* op = reinterpret_cast<T*>(p.o) + row * p.o_token + h * p.o_head;
-  for (int i = 0; i < 4; ++i) {
-    if (lane + 32 * i < p.dim) op[lane + 32 * i] = from_f32<T>(l == 0.0f ? 0.0f : acc[i] / l);
-  }
-  if (p.lse && lane == 0) p.lse[static_cast<int64_t>(row) * p.heads + h] = l == 0.0f ? -INFINITY : m + logf(l);
-}
-
 static ServingProblem make_problem(const fb200_attention_params* p, const void* q, void* o, float* lse, const int32_t* cu_q) {
   ServingProblem r{};
   r.q = static_cast<const uint8_t*>(q);
@@ -118,15 +57,6 @@ static ServingProblem make_problem(const fb200_attention_params* p, const void* 
   r.causal = p->causal != 0;
   r.scale = p->scale;
   return r;
-}
-
-static int launch_rows(const ServingProblem& r, const PagedCache& c, bool paged, bool e4m3, int dtype, cudaStream_t s) {
-  int* status = nullptr;
-  if (int rc = device_status_word(&status)) return rc;
-  const int64_t blocks = (static_cast<int64_t>(r.q_rows) * r.heads + 7) / 8;
-  if (dtype == FB200_BF16) attention_rows_kernel<__nv_bfloat16><<<static_cast<unsigned>(blocks), 256, 0, s>>>(r, c, paged, e4m3, status);
-  else attention_rows_kernel<__half><<<static_cast<unsigned>(blocks), 256, 0, s>>>(r, c, paged, e4m3, status);
-  return after_launch("attention_rows_kernel");
 }
 
 }  // namespace fb200
@@ -157,7 +87,7 @@ extern "C" int fb200_attention_prompt(const fb200_attention_params* params, cons
   r.k_head = params->k_head_stride;
   r.v_token = params->v_token_stride;
   r.v_head = params->v_head_stride;
-  return launch_attention_tiles(r, nullptr, as_stream(stream));
+  return launch_attention_tiles(r, nullptr, false, as_stream(stream));
 }
 
 static int check_paged(const char* what, const fb200_attention_params* p, const fb200_kv_cache* c) {
@@ -199,6 +129,5 @@ extern "C" int fb200_attention_paged(const fb200_attention_params* params, const
   ServingProblem r = make_problem(params, q, o, lse, cu_q);
   r.kv_len = kv_len;
   if (attention_decode_takes(r)) return launch_attention_decode(r, c, cache->dtype == FB200_U8, workspace, as_stream(stream));
-  if (cache->dtype != FB200_U8) return launch_attention_tiles(r, &c, as_stream(stream));
-  return launch_rows(r, c, true, cache->dtype == FB200_U8, params->dtype, as_stream(stream));
+  return launch_attention_tiles(r, &c, cache->dtype == FB200_U8, as_stream(stream));
 }

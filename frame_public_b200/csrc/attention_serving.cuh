@@ -31,7 +31,7 @@ __device__ __forceinline__ void serving_lengths(const ServingProblem& p, const P
   }
 }
 
-int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, cudaStream_t stream);
+int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, bool e4m3, cudaStream_t stream);
 bool attention_decode_takes(const ServingProblem& p);
 size_t attention_decode_workspace(const ServingProblem& p);
 int launch_attention_decode(const ServingProblem& p, const PagedCache& cache, bool e4m3, void* workspace, cudaStream_t stream);

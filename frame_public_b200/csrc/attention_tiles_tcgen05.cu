@@ -29,6 +29,8 @@
 // scores are computed 128 keys at a time (steps of 64 took 584 us where these take 518, 2x8192 d128).
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "attention_serving.cuh"
 #include "sm100_ptx.cuh"
 
@@ -44,7 +46,10 @@ constexpr int kTileRows = 128;
 constexpr int kTileKeys = 128;
 constexpr int kSoftmaxWarps = 16;             // two threads per row of each stage, 64 of the 128 keys each
 constexpr int kMmaWarp = kSoftmaxWarps, kCopyWarp = kSoftmaxWarps + 1;
-constexpr int kTilesThreads = (kSoftmaxWarps + 2) * 32;
+constexpr int kCodeWarps = 3;                 // copy warps of an e4m3 cache (20 warps are five per scheduler, as 18 are)
+__host__ __device__ constexpr int tiles_threads(bool e4m3) { return (kSoftmaxWarps + 1 + (e4m3 ? kCodeWarps : 1)) * 32; }
+__host__ __device__ constexpr int tiles_slots(int spans, bool e4m3) { return spans == 1 ? 8 : e4m3 ? 4 : 5; }
+constexpr int kScaleTiles = 4;                // tiles whose scales are kept: a tile's are read until the scores two tiles on
 constexpr int kHalfKeys = kTileKeys / 2;
 constexpr int kSpanBytes = kTileRows * 128;   // 128 rows of 64 16-bit elements
 constexpr float kRescaleStep = 8.0f;          // log2 of the growth of a row's maximum that O follows at once
@@ -175,8 +180,10 @@ __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int 
   return false;
 }
 
-// Barriers and the swap of row maxima, in front of the tiles.
-__host__ __device__ constexpr uint32_t kTilesSmallBytes(int spans) { return 320 + (spans == 1 ? 2 : 1) * 4 * kTileRows * 4; }
+// Barriers, the swap of row maxima and an e4m3 cache's scales, in front of the tiles.
+__host__ __device__ constexpr uint32_t tiles_small_bytes(int spans, bool e4m3) {
+  return 320 + (spans == 1 ? 2 : 1) * 4 * kTileRows * 4 + (e4m3 ? kScaleTiles * 2 * kTileKeys * 4 : 0);
+}
 
 // A place in the ring; K and V tiles alternate, so each steps by two.
 struct RingPos {
@@ -191,17 +198,19 @@ struct RingPos {
   }
 };
 
-template <typename T, int SPANS, bool PAGED>
-__global__ void __launch_bounds__(kTilesThreads, 1)
+template <typename T, int SPANS, bool PAGED, bool E4M3>
+__global__ void __launch_bounds__(tiles_threads(E4M3), 1)
 attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                        const __grid_constant__ CUtensorMap tmap_v, const ServingProblem p, const PagedCache cache,
-                       int tile_tokens, int box_keys, uint32_t fmt, int* status) {
+                       int tile_tokens, int box_keys, int* status) {
+  using PV = typename std::conditional<E4M3, __nv_bfloat16, T>::type;   // type of P and V
+  constexpr uint32_t kFmt = std::is_same<T, __half>::value ? kFmtF16 : kFmtBF16, kFmtPV = std::is_same<PV, __half>::value ? kFmtF16 : kFmtBF16;
   constexpr int kSlotBytes = SPANS * kSpanBytes;
-  constexpr int kSlots = SPANS == 2 ? 5 : 8;
+  constexpr int kSlots = tiles_slots(SPANS, E4M3);
   constexpr bool kApart = SPANS == 1;   // P has columns of its own
   constexpr uint32_t kTmemO = 2 * kTileKeys, kTmemP = kApart ? kTmemO + 128 : 0, kTmemPStage = kApart ? 64 : kTileKeys;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const uint32_t bars = smem_u32(smem_raw), base = (bars + kTilesSmallBytes(SPANS) + 1023u) & ~1023u;   // swizzle atoms are 1024 bytes
+  const uint32_t bars = smem_u32(smem_raw), base = (bars + tiles_small_bytes(SPANS, E4M3) + 1023u) & ~1023u;   // swizzle atoms are 1024 bytes
   uint8_t* base_ptr = smem_raw + (base - bars);
   const uint32_t q_s = base, ring = base + 2 * kSlotBytes;
   const uint32_t bar_q = bars, full = bars + 8, freed = full + 8 * kSlots, bar_s = freed + 8 * kSlots, bar_r = bar_s + 16,
@@ -211,6 +220,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   TilesItem* const item_ptr = reinterpret_cast<TilesItem*>(after + 16);
   int* const found_ptr = reinterpret_cast<int*>(after + 16 + sizeof(TilesItem));
   float* const share = reinterpret_cast<float*>(smem_raw + 320);   // [tile parity, P apart only][stage][half][row]: maxima, then sums
+  float* const scales = share + (kApart ? 2 : 1) * 4 * kTileRows;          // [tile % kScaleTiles][K, V][key]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.x % p.kv_heads;
@@ -224,7 +234,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   } else if (warp == kMmaWarp && lane == 0) {
     mbar_init(bar_q, 1);
     for (int i = 0; i < kSlots; ++i) {
-      mbar_init(full + 8 * i, 1);
+      mbar_init(full + 8 * i, E4M3 ? kCodeWarps : 1);
       mbar_init(freed + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -260,10 +270,10 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   }
   const int most = max(tiles[0], tiles[1]);   // stage 1's rows come later: it sees as much, unless it has none
 
-  if (warp == kCopyWarp) {
+  if (warp >= kCopyWarp) {
     // ---- copies ----------------------------------------------------------------------------------
     if (most > 0) {
-      if (lane == 0) {
+      if (warp == kCopyWarp && lane == 0) {
         const int live_stages = (tiles[0] > 0) + (tiles[1] > 0);
         mbar_arrive_expect_tx(bar_q, static_cast<uint32_t>(live_stages * tile_tokens * p.group * 128 * SPANS));
         for (int s = 0; s < 2; ++s) {
@@ -275,6 +285,94 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
       __syncwarp();
       bool live = true;
+      if constexpr (E4M3) {
+        // Codes become the operands of the tensor core on their way: 16 at a time from global memory through
+        // registers into the swizzled tile (K in the query's type, V in bfloat16), those of the next tile
+        // fetched before this one's slot is free.  Rows behind the last key become zeros.
+        constexpr int kUnits = SPANS * 4, kMine = (kTileKeys * kUnits + kCodeWarps * 32 - 1) / (kCodeWarps * 32);
+        const int me = (warp - kCopyWarp) * 32 + lane, units = p.dim / 16;
+        // pages of the tile's 16 groups of 8 keys, in lanes 0-15
+        auto pages_of = [&](int j) {
+          const int key = j * kTileKeys + (lane & 15) * 8;
+          return key < item.lk ? cache.table[item.seq * cache.table_stride + (key >> cache.page_shift)] : 0;
+        };
+        auto checked = [&](int page) {
+          if (static_cast<uint32_t>(page) < static_cast<uint32_t>(cache.pages)) return page;
+          record_fault(status, kFaultBadPage);
+          return 0;
+        };
+        uint4 raw[kMine];
+        uint32_t scale_raw[2][2] = {};
+        int page_raw = pages_of(0), page = 0;
+        auto fetch = [&](int n) {
+          const int j = n >> 1;
+          if (!(n & 1)) {
+            page = checked(page_raw);
+            page_raw = pages_of(j + 1);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int row = me + i * (kCodeWarps * 32), key = j * kTileKeys + row;
+              const int pg = __shfl_sync(0xffffffffu, page, (row >> 3) & 15);
+              scale_raw[i][0] = scale_raw[i][1] = 0;
+              if (row < kTileKeys && key < item.lk) {
+                const int64_t at = scale_offset(cache, pg, key, head);
+                scale_raw[i][0] = cache.k_scale[at];
+                scale_raw[i][1] = cache.v_scale[at];
+              }
+            }
+          }
+          const uint8_t* const from = (n & 1) ? cache.v : cache.k;
+#pragma unroll
+          for (int i = 0; i < kMine; ++i) {
+            const int at = me + i * (kCodeWarps * 32), row = at / kUnits, unit = at % kUnits, key = j * kTileKeys + row;
+            const int pg = __shfl_sync(0xffffffffu, page, (row >> 3) & 15);
+            raw[i] = make_uint4(0, 0, 0, 0);
+            if (row < kTileKeys && key < item.lk && unit < units) {
+              raw[i] = *reinterpret_cast<const uint4*>(from + token_offset(cache, pg, key, head) + unit * 16);
+            }
+          }
+        };
+        auto put = [&](int n, uint8_t* slot, auto pair) {
+#pragma unroll
+          for (int i = 0; i < kMine; ++i) {
+            const int at = me + i * (kCodeWarps * 32), row = at / kUnits, unit = at % kUnits;
+            if (row >= kTileKeys) continue;
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int chunk = ((unit & 3) * 2 + e) ^ (row & 7);
+              *reinterpret_cast<uint4*>(slot + (unit >> 2) * kSpanBytes + row * 128 + chunk * 16) =
+                  make_uint4(pair(__byte_perm(w[2 * e], 0, 0x1100)), pair(__byte_perm(w[2 * e], 0, 0x3322)),
+                             pair(__byte_perm(w[2 * e + 1], 0, 0x1100)), pair(__byte_perm(w[2 * e + 1], 0, 0x3322)));
+            }
+          }
+        };
+        fetch(0);
+        for (int n = 0; live && n < 2 * most; ++n) {
+          const int slot = n % kSlots, use = n / kSlots;
+          if (use > 0) live = mbar_wait_lanes(freed + 8 * slot, (use - 1) & 1, status, kFaultTilesRing);
+          if (!live) break;
+          uint8_t* const to = base_ptr + (ring - base) + slot * kSlotBytes;
+          if (n & 1) {
+            put(n, to, [](uint32_t x) { return codes_to_pair<__nv_bfloat16>(x); });
+          } else {
+            put(n, to, [](uint32_t x) { return codes_to_pair<T>(x); });
+            float* const sc = scales + ((n >> 1) % kScaleTiles) * 2 * kTileKeys;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int row = me + i * (kCodeWarps * 32);
+              if (row < kTileKeys) {
+                sc[row] = scale_of_byte(scale_raw[i][0]);
+                sc[kTileKeys + row] = scale_of_byte(scale_raw[i][1]);
+              }
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full + 8 * slot);
+          if (n + 1 < 2 * most) fetch(n + 1);
+        }
+      } else {
       for (int n = 0; live && n < 2 * most; ++n) {   // K and V of tile n / 2 in turn
         const int j = n >> 1, slot = n % kSlots, use = n / kSlots;
         const uint32_t dst = ring + slot * kSlotBytes, bar = full + 8 * slot;
@@ -297,6 +395,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
         }
       }
+      }
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
@@ -306,8 +405,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     // products, three times what the tensor core needs for it).
     if (most > 0) {
       const int k_steps = p.dim / 16;
-      const uint32_t idesc_s = make_instr_desc(fmt, 0, 0, kTileRows, kTileKeys);
-      const uint32_t idesc_o = make_instr_desc(fmt, 0, 1, kTileRows, static_cast<uint32_t>(p.dim));
+      const uint32_t idesc_s = make_instr_desc(kFmt, 0, 0, kTileRows, kTileKeys);
+      const uint32_t idesc_o = make_instr_desc(kFmtPV, 0, 1, kTileRows, static_cast<uint32_t>(p.dim));
       const uint64_t q_desc = make_smem_desc_sw128(q_s, 16, 1024);
       const uint64_t k_desc = make_smem_desc_sw128(ring, 16, 1024);
       const uint64_t v_desc = make_smem_desc(ring, kSpanBytes, 1024, kLayoutSw128);
@@ -365,7 +464,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         live = live && mbar_wait_lanes(full + 8 * vp.slot, vp.phase, status, kFaultTilesKeys);
         if (!live) break;
         const int there = item.lk - j * kTileKeys;
-        if (there < kTileKeys) {
+        if (!E4M3 && there < kTileKeys) {
           // Rows behind the last key hold another sequence's values or none: their P is 0, but 0 times a
           // NaN is not.
           for (int i = lane; i < (kTileKeys - there) * 8 * SPANS; i += 32) {
@@ -426,6 +525,18 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         tcgen05_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_r + 8 * s);
+      }
+      const float* const sc = scales + (j % kScaleTiles) * 2 * kTileKeys + half * kHalfKeys;
+      if constexpr (E4M3) {   // the scale of K is the score's, that of V the probability's
+#pragma unroll
+        for (int i = 0; i < kHalfKeys; i += 4) {
+          const float4 k4 = *reinterpret_cast<const float4*>(sc + i);
+          uint32_t* const x = &r[i >> 5][i & 31];
+          x[0] = __float_as_uint(__uint_as_float(x[0]) * k4.x);
+          x[1] = __float_as_uint(__uint_as_float(x[1]) * k4.y);
+          x[2] = __float_as_uint(__uint_as_float(x[2]) * k4.z);
+          x[3] = __float_as_uint(__uint_as_float(x[3]) * k4.w);
+        }
       }
       const int visible = limit - j * kTileKeys - half * kHalfKeys;
       if (__any_sync(0xffffffffu, visible < kHalfKeys)) {
@@ -489,7 +600,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             x.y = ex2(x.y);
           }
           sum = __fadd2_rn(sum, x);
-          out[e >> 1] = pack_pair<T>(x.x, x.y);
+          if constexpr (E4M3) x = __fmul2_rn(x, *reinterpret_cast<const float2*>(sc + kTileKeys + i * 32 + e));
+          out[e >> 1] = pack_pair<PV>(x.x, x.y);
         }
         tmem_st_32x32b_x16(t_p + i * 16, out);
       }
@@ -546,7 +658,7 @@ static int64_t most_blocks(const ServingProblem& p, int64_t tokens) {
   return by_rows < by_seq ? by_rows : by_seq;
 }
 
-int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, cudaStream_t stream) {
+int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, bool e4m3, cudaStream_t stream) {
   const int tile_tokens = kTileRows / p.group;
   const int64_t grid = most_blocks(p, 2 * tile_tokens) * p.kv_heads;
   if (grid > 0x7fffffff) return set_error(FB200_INVALID_ARGUMENT, "attention: too many tiles");
@@ -557,42 +669,40 @@ int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, cud
   const int qb[4] = {64, p.group, tile_tokens, 1};
   if (int rc = make_tmap_4d(&tq, p.q, p.dtype, qd, qs, qb)) return rc;
   int box_keys = kTileKeys;
+  tk = tv = tq;   // without keys, and for e4m3 codes, nothing is copied through these maps
   if (cache != nullptr) {
     const int64_t page = int64_t(1) << cache->page_shift;
     if (page < box_keys) box_keys = static_cast<int>(page);
-    const int64_t d[4] = {p.dim, page, p.kv_heads, cache->pages > 0 ? cache->pages : 1};
+    const int64_t d[4] = {p.dim, page, p.kv_heads, cache->pages};
     const int64_t st[3] = {cache->token_stride * 2, cache->head_stride * 2, cache->page_stride * 2};
     const int b[4] = {64, box_keys, 1, 1};
-    if (int rc = make_tmap_4d(&tk, cache->pages > 0 ? cache->k : p.q, p.dtype, d, st, b)) return rc;
-    if (int rc = make_tmap_4d(&tv, cache->pages > 0 ? cache->v : p.q, p.dtype, d, st, b)) return rc;
-  } else {
-    const int64_t rows = p.kv_rows > 0 ? p.kv_rows : 1;   // without keys nothing is copied through the maps
-    const int64_t d[4] = {p.dim, rows, p.kv_heads, 1};
+    if (!e4m3 && cache->pages > 0) {
+      if (int rc = make_tmap_4d(&tk, cache->k, p.dtype, d, st, b)) return rc;
+      if (int rc = make_tmap_4d(&tv, cache->v, p.dtype, d, st, b)) return rc;
+    }
+  } else if (p.kv_rows > 0) {
+    const int64_t d[4] = {p.dim, p.kv_rows, p.kv_heads, 1};
     const int64_t ks[3] = {p.k_token * 2, p.k_head * 2, p.k_token * 2}, vs[3] = {p.v_token * 2, p.v_head * 2, p.v_token * 2};
     const int b[4] = {64, box_keys, 1, 1};
-    if (int rc = make_tmap_4d(&tk, p.kv_rows > 0 ? p.k : p.q, p.dtype, d, ks, b)) return rc;
-    if (int rc = make_tmap_4d(&tv, p.kv_rows > 0 ? p.v : p.q, p.dtype, d, vs, b)) return rc;
+    if (int rc = make_tmap_4d(&tk, p.k, p.dtype, d, ks, b)) return rc;
+    if (int rc = make_tmap_4d(&tv, p.v, p.dtype, d, vs, b)) return rc;
   }
   int* status = nullptr;
   if (int rc = device_status_word(&status)) return rc;
-  const size_t smem = ((kTilesSmallBytes(spans) + 1023) & ~1023u) + static_cast<size_t>(spans * kSpanBytes) * (2 + (spans == 2 ? 5 : 8));
-  const PagedCache none{};
-  auto launch = [&](auto kernel, uint32_t fmt) -> int {
+  const PagedCache view = cache != nullptr ? *cache : PagedCache{};
+  auto launch = [&](auto kernel) -> int {
+    const size_t smem = ((tiles_small_bytes(spans, e4m3) + 1023) & ~1023u) + static_cast<size_t>(spans * kSpanBytes) * (2 + tiles_slots(spans, e4m3));
     FB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    kernel<<<static_cast<unsigned>(grid), kTilesThreads, smem, stream>>>(tq, tk, tv, p, cache != nullptr ? *cache : none, tile_tokens,
-                                                                         box_keys, fmt, status);
+    kernel<<<static_cast<unsigned>(grid), tiles_threads(e4m3), smem, stream>>>(tq, tk, tv, p, view, tile_tokens, box_keys, status);
     return FB200_OK;
   };
-  const bool bf = p.dtype == FB200_BF16;
-  int rc = FB200_OK;
-  if (cache != nullptr) {
-    if (spans == 2) rc = bf ? launch(attention_tiles_kernel<__nv_bfloat16, 2, true>, kFmtBF16) : launch(attention_tiles_kernel<__half, 2, true>, kFmtF16);
-    else rc = bf ? launch(attention_tiles_kernel<__nv_bfloat16, 1, true>, kFmtBF16) : launch(attention_tiles_kernel<__half, 1, true>, kFmtF16);
-  } else {
-    if (spans == 2) rc = bf ? launch(attention_tiles_kernel<__nv_bfloat16, 2, false>, kFmtBF16) : launch(attention_tiles_kernel<__half, 2, false>, kFmtF16);
-    else rc = bf ? launch(attention_tiles_kernel<__nv_bfloat16, 1, false>, kFmtBF16) : launch(attention_tiles_kernel<__half, 1, false>, kFmtF16);
-  }
-  if (rc != FB200_OK) return rc;
+  auto pick = [&](auto type) -> int {
+    using T = decltype(type);
+    if (cache == nullptr) return spans == 2 ? launch(attention_tiles_kernel<T, 2, false, false>) : launch(attention_tiles_kernel<T, 1, false, false>);
+    if (e4m3) return spans == 2 ? launch(attention_tiles_kernel<T, 2, true, true>) : launch(attention_tiles_kernel<T, 1, true, true>);
+    return spans == 2 ? launch(attention_tiles_kernel<T, 2, true, false>) : launch(attention_tiles_kernel<T, 1, true, false>);
+  };
+  if (int rc = p.dtype == FB200_BF16 ? pick(__nv_bfloat16()) : pick(__half())) return rc;
   return after_launch("attention_tiles_kernel");
 }
 
