@@ -12,10 +12,10 @@
 //   * A warp streams slabs of keys of its own through a ring of three cp.async stages (8 KiB each at
 //     head_dim 128: 128 KiB in flight per SM) and keeps its own running maximum, sum and O in registers; the
 //     four warps of a CTA meet only at the end of a pair's range, and the ring runs on across it.
-// e4m3 codes are turned into 16-bit operands in registers: K in the query's type (exact), V and P in
-// bfloat16, whose exponent range takes the scale 2^e of any value; the scale of K multiplies the score, that of V
-// the probability.  The contraction index of Q K^T and the columns of O are permuted so that a thread
-// reads 16 codes of one row at a time.
+// e4m3 codes are turned into float16 operands in registers (exact, one conversion per two codes; bfloat16
+// takes five instructions, which bound the kernel: 130 us where this takes TIME_E4M3, 8 sequences over up to
+// 32000 keys); the scale of K multiplies the score, that of V the probability.  The contraction index of
+// Q K^T and the columns of O are permuted so that a thread reads 16 codes of one row at a time.
 #include <type_traits>
 
 #include "attention_serving.cuh"
@@ -30,8 +30,7 @@ constexpr int kDecodeCtasPerSm = 2;
 constexpr int kDecodeMostCtas = kNumSMs * kDecodeCtasPerSm;
 constexpr int kDecodeRows = 16;
 constexpr int kDecodeSlabBytes = 4096;      // K or V of one slab at head_dim 65..128; half below
-constexpr size_t kDecodeCounterBytes = 4096;
-static_assert(kDecodeMostCtas * sizeof(uint32_t) <= kDecodeCounterBytes, "one counter per CTA");
+static_assert(kDecodeMostCtas * sizeof(uint32_t) <= kServingCounterBytes, "one counter per CTA");
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
@@ -124,7 +123,7 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
   constexpr int kUnits = kRowBytes / 16;                   // 16-byte units of a row
   constexpr int kHalf = kSlab * kRowBytes;                 // K or V of a slab
   constexpr int kKeyTiles = kSlab / 8;
-  using PV = typename std::conditional<E4M3, __nv_bfloat16, T>::type;   // type of P and V
+  using M = typename std::conditional<E4M3, __half, T>::type;   // type of the operands
   static_assert(kHalf <= kDecodeSlabBytes, "slab");
 
   extern __shared__ __align__(128) uint8_t smem[];
@@ -202,17 +201,28 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
         page = 0;
       }
       if (valid > 0) {
-#pragma unroll
-        for (int i = 0; i < kSlab * kUnits / 32; ++i) {
-          const int at = i * 32 + lane, row = at / kUnits, unit = at % kUnits;
-          const int pg = __shfl_sync(0xffffffffu, page, row);
+        constexpr int kElem = E4M3 ? 1 : 2, kStepRows = 32 / kUnits;
+        const int row0 = lane / kUnits, unit = lane % kUnits;
+        auto copy = [&](int row, int64_t off) {
           const bool there = row < valid;   // rows behind the last key become zeros
-          const int64_t off = there ? token_offset(cache, pg, key0 + row, load.head) * (E4M3 ? 1 : 2) + unit * 16 : 0;
+          if (!there) off = 0;
           const int swz_k = E4M3 ? (BIG ? (row & 1) << 2 : 0) : row & (kUnits < 8 ? kUnits - 1 : 7);
           const int swz_v = E4M3 ? (BIG ? row & 6 : (row >> 1) & 3) : swz_k;
           if (unit < units) {
             cp_async16(dst + row * kRowBytes + ((unit ^ swz_k) << 4), cache.k + off, there);
             cp_async16(dst + kHalf + row * kRowBytes + ((unit ^ swz_v) << 4), cache.v + off, there);
+          }
+        };
+        if ((1 << cache.page_shift) >= kSlab) {   // a slab lies in one page
+          const int64_t step = cache.token_stride * (kStepRows * kElem);
+          int64_t off = token_offset(cache, __shfl_sync(0xffffffffu, page, 0), key0 + row0, load.head) * kElem + unit * 16;
+#pragma unroll
+          for (int i = 0; i < kSlab / kStepRows; ++i, off += step) copy(row0 + i * kStepRows, off);
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < kSlab / kStepRows; ++i) {
+            const int row = row0 + i * kStepRows;
+            copy(row, token_offset(cache, __shfl_sync(0xffffffffu, page, row), key0 + row, load.head) * kElem + unit * 16);
           }
         }
       }
@@ -251,6 +261,7 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
     const int pair_n = take.tiles;
     uint32_t q[kSteps][4];
     int limit[2];
+    float lift[2] = {c, c};   // of the scores, to the exponent's units
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int r = g4 + half * 8, i = r / p.group;
@@ -270,6 +281,31 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
           if (r < rows && ks < steps) {
             q[ks][half] = *reinterpret_cast<const uint32_t*>(src + (ks * 16 + t * 2) * 2);
             q[ks][half + 2] = *reinterpret_cast<const uint32_t*>(src + (ks * 16 + t * 2 + 8) * 2);
+          }
+        }
+      }
+      if constexpr (E4M3 && !std::is_same<T, __half>::value) {   // bfloat16 rows to float16
+        auto pair = [](uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u)); };
+        float amax = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 f = pair(q[ks][half + 2 * e]);
+            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        float up;
+        lift[half] = c * query_lift(amax, up);
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 f = pair(q[ks][half + 2 * e]);
+            const __half2 h2 = __floats2half2_rn(f.x * up, f.y * up);
+            q[ks][half + 2 * e] = *reinterpret_cast<const uint32_t*>(&h2);
           }
         }
       }
@@ -311,7 +347,7 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
             const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              mma16816<T>(s[n], q[i * 4 + k], codes_to_pair<T>(__byte_perm(w[k], 0, 0x1100)), codes_to_pair<T>(__byte_perm(w[k], 0, 0x3322)));
+              mma16816<M>(s[n], q[i * 4 + k], codes_low(w[k]), codes_high(w[k]));
             }
           }
         }
@@ -324,27 +360,32 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
           if (ks < steps) {
             uint32_t b[4];
             ldmatrix_x4<false>(row_at + (((ks * 2 + ((lane >> 3) & 1)) ^ swz) << 4), b);
-            mma16816<T>(s[0], q[ks], b[0], b[1]);
-            mma16816<T>(s[1], q[ks], b[2], b[3]);
+            mma16816<M>(s[0], q[ks], b[0], b[1]);
+            mma16816<M>(s[1], q[ks], b[2], b[3]);
           }
         }
       }
       // ---- scale, mask, running maximum --------------------------------------------------------------
       float top[2] = {-INFINITY, -INFINITY};
       const bool edge = key0 + kSlab > sure;
+      const float k_factor = scale_of_byte(k_scale), v_factor = scale_of_byte(v_scale), v_exp = scale_exponent(v_scale);   // of key `lane`
 #pragma unroll
       for (int n = 0; n < kKeyTiles; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int key = key0 + n * 8 + t * 2 + e;
-          float f = c;
-          if constexpr (E4M3) f *= scale_of_byte(__shfl_sync(0xffffffffu, k_scale, n * 8 + t * 2 + e));
+          const int at = n * 8 + t * 2 + e, key = key0 + at;
+          float f = 1.0f, weight = 0.0f;
+          if constexpr (E4M3) {
+            f = __shfl_sync(0xffffffffu, k_factor, at);
+            weight = __shfl_sync(0xffffffffu, v_exp, at);
+          }
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            float x = s[n][half * 2 + e] * f;
+            float x = s[n][half * 2 + e] * lift[half];
+            if constexpr (E4M3) x *= f;
             if (edge && key >= limit[half]) x = -INFINITY;
             s[n][half * 2 + e] = x;
-            top[half] = fmaxf(top[half], x);
+            top[half] = fmaxf(top[half], x + weight);
           }
         }
       }
@@ -380,14 +421,13 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
           float e0 = exp2_fast(s[n][half * 2] - base[half]), e1 = exp2_fast(s[n][half * 2 + 1] - base[half]);
           l[half] += e0 + e1;
           if constexpr (E4M3) {
-            const float v0 = scale_of_byte(__shfl_sync(0xffffffffu, v_scale, n * 8 + t * 2));
-            const float v1 = scale_of_byte(__shfl_sync(0xffffffffu, v_scale, n * 8 + t * 2 + 1));
+            const float v0 = __shfl_sync(0xffffffffu, v_factor, n * 8 + t * 2), v1 = __shfl_sync(0xffffffffu, v_factor, n * 8 + t * 2 + 1);
             const int key = key0 + n * 8 + t * 2;
             // a masked key's scale may be NaN
             e0 = edge && key >= limit[half] ? 0.0f : e0 * v0;
             e1 = edge && key + 1 >= limit[half] ? 0.0f : e1 * v1;
           }
-          if constexpr (std::is_same<PV, __half>::value) {
+          if constexpr (std::is_same<M, __half>::value) {
             const __half2 h2 = __floats2half2_rn(e0, e1);
             pa[n >> 1][(n & 1) * 2 + half] = *reinterpret_cast<const uint32_t*>(&h2);
           } else {
@@ -419,10 +459,11 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
             for (int j = 0; j < kWords; ++j) w[i][j] = there ? w[i][j] : 0u;
           }
 #pragma unroll
-          for (int j = 0; j < kCols; ++j) {
-            const uint32_t sel = (j & 3) * 0x11 + (4 + (j & 3)) * 0x1100;   // byte j of the one key, then of the other
-            mma16816<PV>(o[j], pa[k], codes_to_pair<PV>(__byte_perm(w[0][j >> 2], w[1][j >> 2], sel)),
-                         codes_to_pair<PV>(__byte_perm(w[2][j >> 2], w[3][j >> 2], sel)));
+          for (int j = 0; j < kCols; j += 2) {   // bytes j, j + 1 of the one key and of the other, in turn
+            const uint32_t sel = (j & 2) ? 0x7362 : 0x5140;
+            const uint32_t x = __byte_perm(w[0][j >> 2], w[1][j >> 2], sel), y = __byte_perm(w[2][j >> 2], w[3][j >> 2], sel);
+            mma16816<M>(o[j], pa[k], codes_low(x), codes_low(y));
+            mma16816<M>(o[j + 1], pa[k], codes_high(x), codes_high(y));
           }
         }
       } else {
@@ -434,8 +475,8 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
           if (j < steps) {
             uint32_t b[4];
             ldmatrix_x4<true>(row_at + (((j * 2 + (lane >> 4)) ^ swz) << 4), b);
-            mma16816<PV>(o[2 * j], pa[0], b[0], b[1]);
-            mma16816<PV>(o[2 * j + 1], pa[0], b[2], b[3]);
+            mma16816<M>(o[2 * j], pa[0], b[0], b[1]);
+            mma16816<M>(o[2 * j + 1], pa[0], b[2], b[3]);
           }
         }
       }
@@ -459,7 +500,7 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
     const int64_t first_cta = ((pair_t0 + 1) * ctas - 1) / total, last_cta = ((pair_t0 + pair_n) * ctas - 1) / total;
     auto slot_of = [&](int64_t cta) { return 2 * cta + (cta == first_cta && range_start(cta) < pair_t0 ? 1 : 0); };
     const int max_rows = p.max_q * p.group;
-    float* const parts = reinterpret_cast<float*>(workspace + kDecodeCounterBytes);   // [slots][max_rows][dim]
+    float* const parts = reinterpret_cast<float*>(workspace + kServingCounterBytes);   // [slots][max_rows][dim]
     float2* const stats = reinterpret_cast<float2*>(parts + static_cast<int64_t>(2 * gridDim.x) * max_rows * p.dim);
     const int quads = p.dim / 4;
     auto store_row = [&](int r, int d, float4 x, float mr, float lr) {   // the pair's result
@@ -552,7 +593,7 @@ bool attention_decode_takes(const ServingProblem& p) { return static_cast<int64_
 
 size_t attention_decode_workspace(const ServingProblem& p) {
   const size_t rows = static_cast<size_t>(2 * kDecodeMostCtas) * p.max_q * p.group;
-  return kDecodeCounterBytes + rows * p.dim * sizeof(float) + rows * sizeof(float2);
+  return kServingCounterBytes + rows * p.dim * sizeof(float) + rows * sizeof(float2);
 }
 
 int launch_attention_decode(const ServingProblem& p, const PagedCache& cache, bool e4m3, void* workspace, cudaStream_t stream) {

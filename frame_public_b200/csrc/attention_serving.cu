@@ -53,6 +53,7 @@ static ServingProblem make_problem(const fb200_attention_params* p, const void* 
   r.kv_heads = static_cast<int>(p->kv_heads);
   r.dim = static_cast<int>(p->head_dim);
   r.max_q = static_cast<int>(p->max_q < p->q_rows ? p->max_q : p->q_rows);
+  r.max_kv = static_cast<int>(p->max_kv < kMostTokens ? p->max_kv : kMostTokens);
   r.dtype = p->dtype;
   r.causal = p->causal != 0;
   r.scale = p->scale;
@@ -87,7 +88,7 @@ extern "C" int fb200_attention_prompt(const fb200_attention_params* params, cons
   r.k_head = params->k_head_stride;
   r.v_token = params->v_token_stride;
   r.v_head = params->v_head_stride;
-  return launch_attention_tiles(r, nullptr, false, as_stream(stream));
+  return launch_attention_tiles(r, nullptr, false, nullptr, as_stream(stream));
 }
 
 static int check_paged(const char* what, const fb200_attention_params* p, const fb200_kv_cache* c) {
@@ -104,7 +105,7 @@ extern "C" int fb200_attention_paged_workspace(const fb200_attention_params* par
   *bytes = 0;
   if (int rc = check_paged("attention_paged_workspace", params, cache)) return rc;
   const ServingProblem r = make_problem(params, nullptr, nullptr, nullptr, nullptr);
-  if (attention_decode_takes(r)) *bytes = attention_decode_workspace(r);
+  *bytes = attention_decode_takes(r) ? attention_decode_workspace(r) : attention_tiles_workspace(r);
   return FB200_OK;
 }
 
@@ -129,5 +130,5 @@ extern "C" int fb200_attention_paged(const fb200_attention_params* params, const
   ServingProblem r = make_problem(params, q, o, lse, cu_q);
   r.kv_len = kv_len;
   if (attention_decode_takes(r)) return launch_attention_decode(r, c, cache->dtype == FB200_U8, workspace, as_stream(stream));
-  return launch_attention_tiles(r, &c, cache->dtype == FB200_U8, as_stream(stream));
+  return launch_attention_tiles(r, &c, cache->dtype == FB200_U8, workspace, as_stream(stream));
 }

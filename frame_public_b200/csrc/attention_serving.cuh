@@ -15,7 +15,7 @@ struct ServingProblem {
   const int32_t* cu_kv;    // prompt
   const int32_t* kv_len;   // paged
   int64_t q_token, q_head, o_token, o_head, k_token, k_head, v_token, v_head;   // elements
-  int n_seqs, q_rows, kv_rows, heads, kv_heads, group, dim, max_q, causal, dtype;
+  int n_seqs, q_rows, kv_rows, heads, kv_heads, group, dim, max_q, max_kv, causal, dtype;
   float scale;
 };
 
@@ -31,7 +31,11 @@ __device__ __forceinline__ void serving_lengths(const ServingProblem& p, const P
   }
 }
 
-int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, bool e4m3, cudaStream_t stream);
+// The front of every workspace: the decode kernel's counters, zero between calls; no other kernel touches it.
+constexpr size_t kServingCounterBytes = 4096;
+
+int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, bool e4m3, void* workspace, cudaStream_t stream);
+size_t attention_tiles_workspace(const ServingProblem& p);
 bool attention_decode_takes(const ServingProblem& p);
 size_t attention_decode_workspace(const ServingProblem& p);
 int launch_attention_decode(const ServingProblem& p, const PagedCache& cache, bool e4m3, void* workspace, cudaStream_t stream);

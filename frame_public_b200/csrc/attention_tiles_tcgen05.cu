@@ -9,8 +9,9 @@
 //
 // A CTA holds two such tiles ("stages") and walks the keys both see.  Roles:
 //   warps 0-7, 8-15  softmax of stage 0 and 1, two threads per row = TMEM lane with 64 keys each:
-//                    tcgen05.ld of the scores, maximum, exponentials, tcgen05.st of P (16 bit); a quarter of
-//                    the exponentials is a polynomial on the FMA pipe instead of ex2 on the XU pipe
+//                    tcgen05.ld of the scores, maximum, exponentials, tcgen05.st of P (16 bit); an eighth of
+//                    the exponentials is a polynomial on the FMA pipe instead of ex2 on the XU pipe (none:
+//                    134 us where this takes 123, 2x4096 d64; a quarter: 126)
 //   warp 16          every tcgen05.mma: S_s = Q_s K^T (both operands in shared memory), O_s += P_s V with
 //                    P as the A operand in TMEM, so P never passes through shared memory
 //   warp 17          TMA: Q once, K and V tiles through a ring; a paged cache one box per page
@@ -46,9 +47,10 @@ constexpr int kTileRows = 128;
 constexpr int kTileKeys = 128;
 constexpr int kSoftmaxWarps = 16;             // two threads per row of each stage, 64 of the 128 keys each
 constexpr int kMmaWarp = kSoftmaxWarps, kCopyWarp = kSoftmaxWarps + 1;
-constexpr int kCodeWarps = 3;                 // copy warps of an e4m3 cache (20 warps are five per scheduler, as 18 are)
-__host__ __device__ constexpr int tiles_threads(bool e4m3) { return (kSoftmaxWarps + 1 + (e4m3 ? kCodeWarps : 1)) * 32; }
-__host__ __device__ constexpr int tiles_slots(int spans, bool e4m3) { return spans == 1 ? 8 : e4m3 ? 4 : 5; }
+constexpr int kCodeWarp = kCopyWarp + 1, kCodeWarps = 2;   // of an e4m3 cache (20 warps are five per scheduler, as 18 are)
+constexpr int kRawSlots = 3;                  // tiles of codes on their way
+__host__ __device__ constexpr int tiles_threads(bool e4m3) { return (kSoftmaxWarps + 2 + (e4m3 ? kCodeWarps : 0)) * 32; }
+__host__ __device__ constexpr int tiles_slots(int spans, bool e4m3) { return spans == 1 ? (e4m3 ? 6 : 8) : e4m3 ? 3 : 5; }
 constexpr int kScaleTiles = 4;                // tiles whose scales are kept: a tile's are read until the scores two tiles on
 constexpr int kHalfKeys = kTileKeys / 2;
 constexpr int kSpanBytes = kTileRows * 128;   // 128 rows of 64 16-bit elements
@@ -79,12 +81,14 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
   const float2 big = make_float2(12582912.0f, 12582912.0f), t = __fadd2_rn(x, big);
   const float2 n = __fadd2_rn(t, make_float2(-12582912.0f, -12582912.0f));
   const float2 f = __fadd2_rn(x, make_float2(-n.x, -n.y));
-  auto both = [](float a) { return make_float2(a, a); };
-  float2 y = __ffma2_rn(both(0.0013264727f), f, both(0.009671513f));
-  y = __ffma2_rn(y, f, both(0.055507336f));
-  y = __ffma2_rn(y, f, both(0.24022242f));
-  y = __ffma2_rn(y, f, both(0.693147f));
-  y = __ffma2_rn(y, f, both(1.0f));
+  auto poly = [](float z) {   // scalar: the coefficients are immediates, where packed pairs would hold them in registers
+    float y = fmaf(0.0013264727f, z, 0.009671513f);
+    y = fmaf(y, z, 0.055507336f);
+    y = fmaf(y, z, 0.24022242f);
+    y = fmaf(y, z, 0.693147f);
+    return fmaf(y, z, 1.0f);
+  };
+  const float2 y = make_float2(poly(f.x), poly(f.y));
   return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)),
                      __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
 }
@@ -182,8 +186,16 @@ __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int 
 
 // Barriers, the swap of row maxima and an e4m3 cache's scales, in front of the tiles.
 __host__ __device__ constexpr uint32_t tiles_small_bytes(int spans, bool e4m3) {
-  return 320 + (spans == 1 ? 2 : 1) * 4 * kTileRows * 4 + (e4m3 ? kScaleTiles * 2 * kTileKeys * 4 : 0);
+  return 320 + (spans == 1 ? 2 : 1) * 4 * kTileRows * 4 + (e4m3 ? kScaleTiles * 3 * kTileKeys * 4 : 0);
 }
+
+// Few blocks over many keys: the keys of a block go to several CTAs, `tiles` of 128 to each, which leave
+// unnormalised O, maximum (in the exponent's units) and sum for attention_tiles_join_kernel.
+struct TilesSplit {
+  int parts, tiles;   // CTAs per block, tiles per CTA; parts 1: not split
+  float* o;           // [parts][q_rows][heads][dim]
+  float2* stats;      // [parts][q_rows][heads]
+};
 
 // A place in the ring; K and V tiles alternate, so each steps by two.
 struct RingPos {
@@ -202,9 +214,10 @@ template <typename T, int SPANS, bool PAGED, bool E4M3>
 __global__ void __launch_bounds__(tiles_threads(E4M3), 1)
 attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                        const __grid_constant__ CUtensorMap tmap_v, const ServingProblem p, const PagedCache cache,
-                       int tile_tokens, int box_keys, int* status) {
-  using PV = typename std::conditional<E4M3, __nv_bfloat16, T>::type;   // type of P and V
-  constexpr uint32_t kFmt = std::is_same<T, __half>::value ? kFmtF16 : kFmtBF16, kFmtPV = std::is_same<PV, __half>::value ? kFmtF16 : kFmtBF16;
+                       const TilesSplit split, int tile_tokens, int box_keys, int* status) {
+  using M = typename std::conditional<E4M3, __half, T>::type;   // type of the operands
+  constexpr bool kLift = E4M3 && !std::is_same<T, __half>::value;   // the query rows become float16
+  constexpr uint32_t kFmt = std::is_same<M, __half>::value ? kFmtF16 : kFmtBF16;
   constexpr int kSlotBytes = SPANS * kSpanBytes;
   constexpr int kSlots = tiles_slots(SPANS, E4M3);
   constexpr bool kApart = SPANS == 1;   // P has columns of its own
@@ -214,19 +227,20 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   uint8_t* base_ptr = smem_raw + (base - bars);
   const uint32_t q_s = base, ring = base + 2 * kSlotBytes;
   const uint32_t bar_q = bars, full = bars + 8, freed = full + 8 * kSlots, bar_s = freed + 8 * kSlots, bar_r = bar_s + 16,
-                 bar_p = bar_r + 16, bar_o = bar_p + 32, tmem_slot = bar_o + 16;
+                 bar_p = bar_r + 16, bar_o = bar_p + 32, raw_full = bar_o + 16, raw_freed = raw_full + 8 * kRawSlots, bar_lift = raw_freed + 8 * kRawSlots, tmem_slot = bar_lift + 8;
+  const uint32_t raw_ring = ring + kSlots * kSlotBytes;
   uint8_t* const after = smem_raw + (tmem_slot - bars);
   volatile uint32_t* const tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(after);
   TilesItem* const item_ptr = reinterpret_cast<TilesItem*>(after + 16);
   int* const found_ptr = reinterpret_cast<int*>(after + 16 + sizeof(TilesItem));
   float* const share = reinterpret_cast<float*>(smem_raw + 320);   // [tile parity, P apart only][stage][half][row]: maxima, then sums
-  float* const scales = share + (kApart ? 2 : 1) * 4 * kTileRows;          // [tile % kScaleTiles][K, V][key]
+  float* const scales = share + (kApart ? 2 : 1) * 4 * kTileRows;          // [tile % kScaleTiles][K, V, exponent of V][key]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int head = blockIdx.x % p.kv_heads;
+  const int part = blockIdx.x % split.parts, pair = blockIdx.x / split.parts, head = pair % p.kv_heads;
   if (warp == 0) {
     TilesItem it;
-    const bool found = find_item<PAGED>(p, cache, blockIdx.x / p.kv_heads, 2 * tile_tokens, it, status);
+    const bool found = find_item<PAGED>(p, cache, pair / p.kv_heads, 2 * tile_tokens, it, status);
     if (lane == 0) {
       if (found) *item_ptr = it;
       *found_ptr = found;
@@ -244,6 +258,11 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       mbar_init(bar_p + 16 * i + 8, 4);
       mbar_init(bar_o + 8 * i, 1);
     }
+    mbar_init(bar_lift, kSoftmaxWarps);
+    for (int i = 0; E4M3 && i < kRawSlots; ++i) {
+      mbar_init(raw_full + 8 * i, 1);
+      mbar_init(raw_freed + 8 * i, kCodeWarps);
+    }
     mbar_fence_init();
   } else if (warp == kCopyWarp) {
     tmem_alloc(tmem_slot, 512);
@@ -258,22 +277,32 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   const uint32_t tmem = __reduce_max_sync(0xffffffffu, *tmem_slot_ptr);
   const TilesItem item{uniform(item_ptr->seq), uniform(item_ptr->block), uniform(item_ptr->q0),
                        uniform(item_ptr->lq), uniform(item_ptr->k0), uniform(item_ptr->lk)};
-  const bool work = uniform(*found_ptr) != 0;
+  const bool found = uniform(*found_ptr) != 0;
   const int token0 = item.block * 2 * tile_tokens;
-  int tiles[2];
+  int tiles[2];   // of keys that each stage's rows see
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     const int first = token0 + s * tile_tokens;
-    tiles[s] = work && first < item.lq
+    tiles[s] = found && first < item.lq
                    ? (keys_seen(p.causal, min(item.lq, first + tile_tokens), item.lq, item.lk) + kTileKeys - 1) / kTileKeys
                    : 0;
   }
-  const int most = max(tiles[0], tiles[1]);   // stage 1's rows come later: it sees as much, unless it has none
+  const int all = max(tiles[0], tiles[1]);   // stage 1's rows come later: it sees as much, unless it has none
+  // this CTA's part of them
+  const bool parted = split.parts > 1 && all > split.tiles;
+  const int tile0 = part * split.tiles, key0 = tile0 * kTileKeys;
+  const bool work = found && (part == 0 || tile0 < all);
+  if (split.parts > 1) {
+    const int room = part == split.parts - 1 ? 0x7fffffff : split.tiles;   // the last part takes what max_kv did not foresee
+    tiles[0] = max(0, min(tiles[0] - tile0, room));
+    tiles[1] = max(0, min(tiles[1] - tile0, room));
+  }
+  const int most = max(tiles[0], tiles[1]);
 
-  if (warp >= kCopyWarp) {
+  if (warp == kCopyWarp) {
     // ---- copies ----------------------------------------------------------------------------------
     if (most > 0) {
-      if (warp == kCopyWarp && lane == 0) {
+      if (lane == 0) {
         const int live_stages = (tiles[0] > 0) + (tiles[1] > 0);
         mbar_arrive_expect_tx(bar_q, static_cast<uint32_t>(live_stages * tile_tokens * p.group * 128 * SPANS));
         for (int s = 0; s < 2; ++s) {
@@ -285,99 +314,14 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
       __syncwarp();
       bool live = true;
-      if constexpr (E4M3) {
-        // Codes become the operands of the tensor core on their way: 16 at a time from global memory through
-        // registers into the swizzled tile (K in the query's type, V in bfloat16), those of the next tile
-        // fetched before this one's slot is free.  Rows behind the last key become zeros.
-        constexpr int kUnits = SPANS * 4, kMine = (kTileKeys * kUnits + kCodeWarps * 32 - 1) / (kCodeWarps * 32);
-        const int me = (warp - kCopyWarp) * 32 + lane, units = p.dim / 16;
-        // pages of the tile's 16 groups of 8 keys, in lanes 0-15
-        auto pages_of = [&](int j) {
-          const int key = j * kTileKeys + (lane & 15) * 8;
-          return key < item.lk ? cache.table[item.seq * cache.table_stride + (key >> cache.page_shift)] : 0;
-        };
-        auto checked = [&](int page) {
-          if (static_cast<uint32_t>(page) < static_cast<uint32_t>(cache.pages)) return page;
-          record_fault(status, kFaultBadPage);
-          return 0;
-        };
-        uint4 raw[kMine];
-        uint32_t scale_raw[2][2] = {};
-        int page_raw = pages_of(0), page = 0;
-        auto fetch = [&](int n) {
-          const int j = n >> 1;
-          if (!(n & 1)) {
-            page = checked(page_raw);
-            page_raw = pages_of(j + 1);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int row = me + i * (kCodeWarps * 32), key = j * kTileKeys + row;
-              const int pg = __shfl_sync(0xffffffffu, page, (row >> 3) & 15);
-              scale_raw[i][0] = scale_raw[i][1] = 0;
-              if (row < kTileKeys && key < item.lk) {
-                const int64_t at = scale_offset(cache, pg, key, head);
-                scale_raw[i][0] = cache.k_scale[at];
-                scale_raw[i][1] = cache.v_scale[at];
-              }
-            }
-          }
-          const uint8_t* const from = (n & 1) ? cache.v : cache.k;
-#pragma unroll
-          for (int i = 0; i < kMine; ++i) {
-            const int at = me + i * (kCodeWarps * 32), row = at / kUnits, unit = at % kUnits, key = j * kTileKeys + row;
-            const int pg = __shfl_sync(0xffffffffu, page, (row >> 3) & 15);
-            raw[i] = make_uint4(0, 0, 0, 0);
-            if (row < kTileKeys && key < item.lk && unit < units) {
-              raw[i] = *reinterpret_cast<const uint4*>(from + token_offset(cache, pg, key, head) + unit * 16);
-            }
-          }
-        };
-        auto put = [&](int n, uint8_t* slot, auto pair) {
-#pragma unroll
-          for (int i = 0; i < kMine; ++i) {
-            const int at = me + i * (kCodeWarps * 32), row = at / kUnits, unit = at % kUnits;
-            if (row >= kTileKeys) continue;
-            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int chunk = ((unit & 3) * 2 + e) ^ (row & 7);
-              *reinterpret_cast<uint4*>(slot + (unit >> 2) * kSpanBytes + row * 128 + chunk * 16) =
-                  make_uint4(pair(__byte_perm(w[2 * e], 0, 0x1100)), pair(__byte_perm(w[2 * e], 0, 0x3322)),
-                             pair(__byte_perm(w[2 * e + 1], 0, 0x1100)), pair(__byte_perm(w[2 * e + 1], 0, 0x3322)));
-            }
-          }
-        };
-        fetch(0);
-        for (int n = 0; live && n < 2 * most; ++n) {
-          const int slot = n % kSlots, use = n / kSlots;
-          if (use > 0) live = mbar_wait_lanes(freed + 8 * slot, (use - 1) & 1, status, kFaultTilesRing);
-          if (!live) break;
-          uint8_t* const to = base_ptr + (ring - base) + slot * kSlotBytes;
-          if (n & 1) {
-            put(n, to, [](uint32_t x) { return codes_to_pair<__nv_bfloat16>(x); });
-          } else {
-            put(n, to, [](uint32_t x) { return codes_to_pair<T>(x); });
-            float* const sc = scales + ((n >> 1) % kScaleTiles) * 2 * kTileKeys;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int row = me + i * (kCodeWarps * 32);
-              if (row < kTileKeys) {
-                sc[row] = scale_of_byte(scale_raw[i][0]);
-                sc[kTileKeys + row] = scale_of_byte(scale_raw[i][1]);
-              }
-            }
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full + 8 * slot);
-          if (n + 1 < 2 * most) fetch(n + 1);
-        }
-      } else {
-      for (int n = 0; live && n < 2 * most; ++n) {   // K and V of tile n / 2 in turn
-        const int j = n >> 1, slot = n % kSlots, use = n / kSlots;
-        const uint32_t dst = ring + slot * kSlotBytes, bar = full + 8 * slot;
+      // K and V of tile n / 2 in turn: into the ring, or as codes into the raw ring
+      constexpr int kInto = E4M3 ? kRawSlots : kSlots, kIntoBytes = E4M3 ? kSpanBytes : kSlotBytes, kBoxes = E4M3 ? 1 : SPANS;
+      const uint32_t into = E4M3 ? raw_ring : ring, into_full = E4M3 ? raw_full : full, into_freed = E4M3 ? raw_freed : freed;
+      for (int n = 0; live && n < 2 * most; ++n) {
+        const int slot = n % kInto, use = n / kInto;
+        const uint32_t dst = into + slot * kIntoBytes, bar = into_full + 8 * slot;
         const void* map = (n & 1) ? static_cast<const void*>(&tmap_v) : &tmap_k;
-        const int key = j * kTileKeys + lane * box_keys;
+        const int key = key0 + (n >> 1) * kTileKeys + lane * box_keys;
         const bool mine = lane * box_keys < kTileKeys && (!PAGED || key < item.lk);
         const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
         int page = 0, row = item.k0 + key;
@@ -385,16 +329,99 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           page = page_number(cache, item.seq, key >> cache.page_shift, status);
           row = key & ((1 << cache.page_shift) - 1);
         }
-        if (use > 0) live = mbar_wait_lanes(freed + 8 * slot, (use - 1) & 1, status, kFaultTilesRing);
+        if (use > 0) live = mbar_wait_lanes(into_freed + 8 * slot, (use - 1) & 1, status, kFaultTilesRing);
         if (!live) break;
-        if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(boxes * box_keys * 128 * SPANS));
+        if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(boxes * box_keys * 128 * kBoxes));
         __syncwarp();
         if (mine) {
-          for (int x = 0; x < SPANS; ++x) {
+          for (int x = 0; x < kBoxes; ++x) {
             tma_load_4d(dst + x * kSpanBytes + lane * box_keys * 128, map, bar, x * 64, row, head, page);
           }
         }
       }
+    }
+    __syncwarp();
+  } else if (E4M3 && warp >= kCodeWarp) {
+    // ---- codes into float16 operands, rows behind the last key zero ------------------------------------
+    if constexpr (E4M3) {
+      constexpr int kUnits = SPANS * 4;   // 16 codes each
+      const int me = (warp - kCodeWarp) * 32 + lane;
+      // Scale bytes of keys me and me + 64, fetched one tile ahead, and the pages they lie in, two tiles ahead.
+      int page_raw[2] = {0, 0};
+      uint32_t k_scale[2], v_scale[2], k_scale_next[2], v_scale_next[2];
+      auto pages_ahead = [&](int first) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int key = first + me + i * 64;
+          page_raw[i] = key < item.lk ? cache.table[item.seq * cache.table_stride + (key >> cache.page_shift)] : 0;
+        }
+      };
+      auto scales_ahead = [&](int first) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int key = first + me + i * 64;
+          k_scale_next[i] = v_scale_next[i] = 0;
+          if (key < item.lk) {   // (a page outside the cache is recorded by the copy warp)
+            const int page = static_cast<uint32_t>(page_raw[i]) < static_cast<uint32_t>(cache.pages) ? page_raw[i] : 0;
+            const int64_t at = scale_offset(cache, page, key, head);
+            k_scale_next[i] = cache.k_scale[at];
+            v_scale_next[i] = cache.v_scale[at];
+          }
+        }
+      };
+      if (most > 0) {
+        pages_ahead(key0);
+        scales_ahead(key0);
+        pages_ahead(key0 + kTileKeys);
+      }
+      bool live = true;
+      for (int n = 0; live && n < 2 * most; ++n) {
+        const int slot = n % kSlots, use = n / kSlots, from = n % kRawSlots, key_tile = key0 + (n >> 1) * kTileKeys;
+        if (!(n & 1)) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            k_scale[i] = k_scale_next[i];
+            v_scale[i] = v_scale_next[i];
+          }
+          scales_ahead(key_tile + kTileKeys);
+          pages_ahead(key_tile + 2 * kTileKeys);
+        }
+        if (use > 0) live = mbar_wait_lanes(freed + 8 * slot, (use - 1) & 1, status, kFaultTilesRing);
+        live = live && mbar_wait_lanes(raw_full + 8 * from, (n / kRawSlots) & 1, status, kFaultTilesKeys);
+        if (!live) break;
+        uint8_t* const to = base_ptr + (ring - base) + slot * kSlotBytes;
+        const uint8_t* const raw = base_ptr + (raw_ring - base) + from * kSpanBytes;
+        auto convert = [&] {
+#pragma unroll 4
+          for (int i = 0; i < kTileKeys * kUnits / (kCodeWarps * 32); ++i) {
+            const int at = me + i * (kCodeWarps * 32), row = at / kUnits, unit = at % kUnits;
+            uint4 c = *reinterpret_cast<const uint4*>(raw + row * 128 + ((unit ^ (row & 7)) << 4));
+            if (key_tile + row >= item.lk) c = make_uint4(0, 0, 0, 0);
+            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int chunk = ((unit & 3) * 2 + e) ^ (row & 7);
+              *reinterpret_cast<uint4*>(to + (unit >> 2) * kSpanBytes + row * 128 + chunk * 16) =
+                  make_uint4(codes_low(w[2 * e]), codes_high(w[2 * e]), codes_low(w[2 * e + 1]), codes_high(w[2 * e + 1]));
+            }
+          }
+        };
+        convert();
+        if (!(n & 1)) {
+          float* const sc = scales + ((n >> 1) % kScaleTiles) * 3 * kTileKeys;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            sc[me + i * 64] = scale_of_byte(k_scale[i]);
+            sc[kTileKeys + me + i * 64] = scale_of_byte(v_scale[i]);
+            sc[2 * kTileKeys + me + i * 64] = scale_exponent(v_scale[i]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(raw_freed + 8 * from);
+          mbar_arrive(full + 8 * slot);
+        }
       }
     }
     __syncwarp();
@@ -406,11 +433,12 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     if (most > 0) {
       const int k_steps = p.dim / 16;
       const uint32_t idesc_s = make_instr_desc(kFmt, 0, 0, kTileRows, kTileKeys);
-      const uint32_t idesc_o = make_instr_desc(kFmtPV, 0, 1, kTileRows, static_cast<uint32_t>(p.dim));
+      const uint32_t idesc_o = make_instr_desc(kFmt, 0, 1, kTileRows, static_cast<uint32_t>(p.dim));
       const uint64_t q_desc = make_smem_desc_sw128(q_s, 16, 1024);
       const uint64_t k_desc = make_smem_desc_sw128(ring, 16, 1024);
       const uint64_t v_desc = make_smem_desc(ring, kSpanBytes, 1024, kLayoutSw128);
-      bool live = mbar_wait_lanes(bar_q, 0, status, kFaultTilesQuery);
+      bool live = mbar_wait_lanes(kLift ? bar_lift : bar_q, 0, status, kFaultTilesQuery);
+      if constexpr (kLift) tcgen05_fence_after_sync();
       RingPos kp{0, 0}, vp{1, 0};   // of the K and the V tile that come next
       auto scores = [&](int s) {
         const uint64_t a = q_desc + static_cast<uint64_t>(s * (kSlotBytes / 16)), b = k_desc + static_cast<uint64_t>(kp.slot * (kSlotBytes / 16));
@@ -463,7 +491,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         }
         live = live && mbar_wait_lanes(full + 8 * vp.slot, vp.phase, status, kFaultTilesKeys);
         if (!live) break;
-        const int there = item.lk - j * kTileKeys;
+        const int there = item.lk - key0 - j * kTileKeys;
         if (!E4M3 && there < kTileKeys) {
           // Rows behind the last key hold another sequence's values or none: their P is 0, but 0 times a
           // NaN is not.
@@ -496,7 +524,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     const int in_tile = row / p.group, token = token0 + s * tile_tokens + in_tile;
     const int h = head * p.group + row - in_tile * p.group;
     const bool there = work && in_tile < tile_tokens && token < item.lq;
-    const int limit = there ? keys_seen(p.causal, token + 1, item.lq, item.lk) : 0;   // keys this row sees
+    const int limit = there ? keys_seen(p.causal, token + 1, item.lq, item.lk) - key0 : 0;   // keys this row sees from key0 on
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t t_s = lanes + s * kTileKeys + half * kHalfKeys, t_p = lanes + kTmemP + s * kTmemPStage + half * (kHalfKeys / 2);
     const uint32_t t_o = lanes + kTmemO + s * (SPANS * 64);
@@ -510,9 +538,42 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                    : "=r"(all) : "r"(1 + s * 4 + (warp & 3)), "r"(ok ? 1u : 0u) : "memory");
       return all != 0;
     };
-    const float c = p.scale * 1.4426950408889634f;
-    float m = -INFINITY, l = 0.0f;
+    float c = p.scale * 1.4426950408889634f, m = -INFINITY, l = 0.0f;
     bool live = true;
+    if constexpr (kLift) {   // this half of the row to float16, in place
+      uint4* const q_row = reinterpret_cast<uint4*>(base_ptr + s * kSlotBytes + row * 128 + half * (SPANS == 2 ? kSpanBytes : 64));
+      float amax = 0.0f;
+      if (tiles[s] > 0) {
+        live = mbar_wait_lanes(bar_q, 0, status, kFaultTilesQuery);
+#pragma unroll
+        for (int i = 0; i < SPANS * 4; ++i) {
+          const uint4 x = q_row[i];
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xFFFF0000u))));
+        }
+      }
+      *mine = amax;
+      live = pair_sync(live);
+      amax = fmaxf(amax, *other);
+      live = pair_sync(live);   // read before it is written again
+      float up;
+      c *= query_lift(amax, up);
+      if (tiles[s] > 0) {
+#pragma unroll
+        for (int i = 0; i < SPANS * 4; ++i) {
+          const uint4 x = q_row[i];
+          uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = pack_pair<__half>(__uint_as_float(w[e] << 16) * up, __uint_as_float(w[e] & 0xFFFF0000u) * up);
+          q_row[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_lift);
+    }
+    const float to_exp = E4M3 ? 1.0f : c;   // of the maximum and the scores below to the exponent's units
     for (int j = 0; j < tiles[s]; ++j) {
       live = mbar_wait_lanes(bar_s + 8 * s, j & 1, status, kFaultTilesScores);
       tcgen05_fence_after_sync();
@@ -526,16 +587,16 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_r + 8 * s);
       }
-      const float* const sc = scales + (j % kScaleTiles) * 2 * kTileKeys + half * kHalfKeys;
+      const float* const sc = scales + (j % kScaleTiles) * 3 * kTileKeys + half * kHalfKeys;
       if constexpr (E4M3) {   // the scale of K is the score's, that of V the probability's
+        const float2 c2 = make_float2(c, c);
 #pragma unroll
         for (int i = 0; i < kHalfKeys; i += 4) {
           const float4 k4 = *reinterpret_cast<const float4*>(sc + i);
           uint32_t* const x = &r[i >> 5][i & 31];
-          x[0] = __float_as_uint(__uint_as_float(x[0]) * k4.x);
-          x[1] = __float_as_uint(__uint_as_float(x[1]) * k4.y);
-          x[2] = __float_as_uint(__uint_as_float(x[2]) * k4.z);
-          x[3] = __float_as_uint(__uint_as_float(x[3]) * k4.w);
+          const float2 lo = __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), c2), make_float2(k4.x, k4.y));
+          const float2 hi = __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(x[2]), __uint_as_float(x[3])), c2), make_float2(k4.z, k4.w));
+          x[0] = __float_as_uint(lo.x), x[1] = __float_as_uint(lo.y), x[2] = __float_as_uint(hi.x), x[3] = __float_as_uint(hi.y);
         }
       }
       const int visible = limit - j * kTileKeys - half * kHalfKeys;
@@ -547,7 +608,13 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < kHalfKeys; i += 2) {
+      for (int i = 0; E4M3 && i < kHalfKeys; i += 2) {   // of probability times value scale: see kScaleFloor
+        const float2 x = __fadd2_rn(make_float2(__uint_as_float(r[i >> 5][i & 31]), __uint_as_float(r[i >> 5][(i & 31) + 1])),
+                                    *reinterpret_cast<const float2*>(sc + 2 * kTileKeys + i));
+        top[(i >> 1) & 3] = fmaxf(top[(i >> 1) & 3], fmaxf(x.x, x.y));
+      }
+#pragma unroll
+      for (int i = 0; !E4M3 && i < kHalfKeys; i += 2) {
         top[(i >> 1) & 3] = fmaxf(top[(i >> 1) & 3], fmaxf(__uint_as_float(r[i >> 5][i & 31]), __uint_as_float(r[i >> 5][(i & 31) + 1])));
       }
       float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
@@ -569,9 +636,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       mx = fmaxf(mx, other[swap]);
       if (j == 0) {
         m = mx;
-      } else if (__any_sync(0xffffffffu, (mx - m) * c > kRescaleStep)) {   // -inf - -inf compares false
+      } else if (__any_sync(0xffffffffu, (mx - m) * to_exp > kRescaleStep)) {   // -inf - -inf compares false
         const float next = fmaxf(m, mx);
-        const float f = next == -INFINITY ? 1.0f : ex2((m - next) * c);
+        const float f = next == -INFINITY ? 1.0f : ex2((m - next) * to_exp);
         m = next;
         l *= f;
         // the first half's threads do it, whose P the tensor core waits for before anything else
@@ -584,7 +651,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           tmem_st_32x32b_x16(t_o + i, x);
         }
       }
-      const float mc = m == -INFINITY ? 0.0f : m * c;
+      const float mc = m == -INFINITY ? 0.0f : m * to_exp;
       float2 sum = make_float2(0.0f, 0.0f);
       const float2 c2 = make_float2(c, c), nm2 = make_float2(-mc, -mc);
 #pragma unroll
@@ -592,8 +659,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         uint32_t out[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          float2 x = __ffma2_rn(make_float2(__uint_as_float(r[i][e]), __uint_as_float(r[i][e + 1])), c2, nm2);
-          if ((e & 7) == 6) {
+          float2 x = make_float2(__uint_as_float(r[i][e]), __uint_as_float(r[i][e + 1]));
+          x = E4M3 ? __fadd2_rn(x, nm2) : __ffma2_rn(x, c2, nm2);
+          if ((e & 15) == 14) {
             x = exp2_poly(x);
           } else {
             x.x = ex2(x.x);
@@ -601,7 +669,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
           sum = __fadd2_rn(sum, x);
           if constexpr (E4M3) x = __fmul2_rn(x, *reinterpret_cast<const float2*>(sc + kTileKeys + i * 32 + e));
-          out[e >> 1] = pack_pair<PV>(x.x, x.y);
+          out[e >> 1] = pack_pair<M>(x.x, x.y);
         }
         tmem_st_32x32b_x16(t_p + i * 16, out);
       }
@@ -621,6 +689,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     if (live) {
       tcgen05_fence_after_sync();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int64_t at = static_cast<int64_t>(item.q0 + token) * p.heads + h;
       T* const dst = reinterpret_cast<T*>(p.o) + static_cast<int64_t>(item.q0 + token) * p.o_token + h * p.o_head;
       for (int i = half * 16; i < p.dim; i += 32) {
         uint32_t x[16];
@@ -628,7 +697,12 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           tmem_ld_32x32b_x16(t_o + i, x);
           tmem_ld_wait(x);
         }
-        if (there) {
+        if (!there) continue;
+        if (parted) {
+          float* const to = split.o + (part * static_cast<int64_t>(p.q_rows) * p.heads + at) * p.dim + i;
+#pragma unroll
+          for (int e = 0; any && e < 16; e += 4) *reinterpret_cast<uint4*>(to + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        } else {
           uint32_t out[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -638,8 +712,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           *reinterpret_cast<uint4*>(dst + i + 8) = make_uint4(out[4], out[5], out[6], out[7]);
         }
       }
-      if (there && half == 0 && p.lse != nullptr) {
-        p.lse[static_cast<int64_t>(item.q0 + token) * p.heads + h] = l == 0.0f ? -INFINITY : m * p.scale + logf(l);
+      if (there && half == 0) {
+        if (parted) split.stats[part * static_cast<int64_t>(p.q_rows) * p.heads + at] = make_float2(any ? m * to_exp : -INFINITY, l);
+        else if (p.lse != nullptr) p.lse[at] = l == 0.0f ? -INFINITY : m * to_exp * 0.6931471805599453f + logf(l);
       }
     }
   }
@@ -651,6 +726,52 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   }
 }
 
+// Joins the parts of split blocks in the order of the keys: one warp per (row, head).
+template <typename T>
+__global__ void __launch_bounds__(256) attention_tiles_join_kernel(const ServingProblem p, const PagedCache cache, const TilesSplit split,
+                                                                   int tile_tokens) {
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (at >= static_cast<int64_t>(p.q_rows) * p.heads) return;
+  const int row = static_cast<int>(at / p.heads), h = static_cast<int>(at - static_cast<int64_t>(row) * p.heads);
+  const int s = sequence_of_row(p.cu_q, p.n_seqs, row);
+  if (s < 0) return;
+  int q0, lq, k0, lk;
+  serving_lengths<true>(p, cache, s, q0, lq, k0, lk);
+  const int end = min(lq, ((row - q0) / (2 * tile_tokens) + 1) * 2 * tile_tokens);   // of the row's block
+  const int tiles = (keys_seen(p.causal, end, lq, lk) + kTileKeys - 1) / kTileKeys;
+  if (tiles <= split.tiles) return;   // written by its CTA
+  const int parts = min(split.parts, (tiles + split.tiles - 1) / split.tiles);
+  const int64_t stride = static_cast<int64_t>(p.q_rows) * p.heads;
+  float m = -INFINITY;
+  for (int i = lane; i < parts; i += 32) m = fmaxf(m, split.stats[i * stride + at].x);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  float4 sum = make_float4(0, 0, 0, 0);
+  float l = 0.0f;
+  const bool mine = lane * 4 < p.dim;
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float2 ml = split.stats[i * stride + at];
+    if (ml.x == -INFINITY) continue;   // saw no key: nothing was stored
+    const float f = ex2(ml.x - m);
+    l += f * ml.y;
+    if (mine) {
+      const float4 x = *reinterpret_cast<const float4*>(split.o + (i * stride + at) * p.dim + lane * 4);
+      sum.x += f * x.x;
+      sum.y += f * x.y;
+      sum.z += f * x.z;
+      sum.w += f * x.w;
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (mine) {
+    const uint2 out = l == 0.0f ? make_uint2(0, 0) : make_uint2(pack_pair<T>(sum.x * inv, sum.y * inv), pack_pair<T>(sum.z * inv, sum.w * inv));
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + static_cast<int64_t>(row) * p.o_token + h * p.o_head + lane * 4) = out;
+  }
+  if (lane == 0 && p.lse != nullptr) p.lse[at] = l == 0.0f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+}
+
 // Blocks of `tokens` query tokens there can be.
 static int64_t most_blocks(const ServingProblem& p, int64_t tokens) {
   const int64_t by_rows = p.q_rows / tokens + p.n_seqs;
@@ -658,9 +779,37 @@ static int64_t most_blocks(const ServingProblem& p, int64_t tokens) {
   return by_rows < by_seq ? by_rows : by_seq;
 }
 
-int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, bool e4m3, cudaStream_t stream) {
+// How a call over a cache is split.  A block per SM or more is left whole (cutting 256 blocks of up to 94
+// tiles cost 248 us against 216: partial results of every row for little better balance); with fewer the
+// keys are cut into parts of at least eight tiles (1024 keys) so that there are about two CTAs per SM,
+// whatever the lengths are: short sequences simply have fewer parts (16 sequences of 5 new tokens over up
+// to 8000 keys: 127 -> 78 us, one such sequence 124 -> 33 us).
+static void tiles_split_shape(const ServingProblem& p, int& parts, int& tiles) {
+  const int64_t blocks = most_blocks(p, 2 * (kTileRows / p.group)) * p.kv_heads, all = (static_cast<int64_t>(p.max_kv) + kTileKeys - 1) / kTileKeys;
+  parts = 1;
+  tiles = 0;
+  if (blocks == 0 || blocks >= kNumSMs || all <= 8) return;
+  const int64_t each = (all * blocks + 2 * kNumSMs - 1) / (2 * kNumSMs);
+  tiles = static_cast<int>(each < 8 ? 8 : each);
+  parts = static_cast<int>((all + tiles - 1) / tiles);
+}
+
+size_t attention_tiles_workspace(const ServingProblem& p) {
+  int parts, tiles;
+  tiles_split_shape(p, parts, tiles);
+  if (parts == 1) return 0;
+  return kServingCounterBytes + static_cast<size_t>(parts) * p.q_rows * p.heads * (static_cast<size_t>(p.dim) * sizeof(float) + sizeof(float2));
+}
+
+int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, bool e4m3, void* workspace, cudaStream_t stream) {
   const int tile_tokens = kTileRows / p.group;
-  const int64_t grid = most_blocks(p, 2 * tile_tokens) * p.kv_heads;
+  TilesSplit split{1, 0, nullptr, nullptr};
+  if (cache != nullptr) {
+    tiles_split_shape(p, split.parts, split.tiles);
+    split.o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kServingCounterBytes);
+    split.stats = reinterpret_cast<float2*>(split.o + static_cast<size_t>(split.parts) * p.q_rows * p.heads * p.dim);
+  }
+  const int64_t grid = most_blocks(p, 2 * tile_tokens) * p.kv_heads * split.parts;
   if (grid > 0x7fffffff) return set_error(FB200_INVALID_ARGUMENT, "attention: too many tiles");
   if (grid == 0) return FB200_OK;
   const int spans = p.dim > 64 ? 2 : 1;
@@ -669,16 +818,17 @@ int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, boo
   const int qb[4] = {64, p.group, tile_tokens, 1};
   if (int rc = make_tmap_4d(&tq, p.q, p.dtype, qd, qs, qb)) return rc;
   int box_keys = kTileKeys;
-  tk = tv = tq;   // without keys, and for e4m3 codes, nothing is copied through these maps
+  tk = tv = tq;   // without keys nothing is copied through these maps
   if (cache != nullptr) {
     const int64_t page = int64_t(1) << cache->page_shift;
     if (page < box_keys) box_keys = static_cast<int>(page);
     const int64_t d[4] = {p.dim, page, p.kv_heads, cache->pages};
     const int64_t st[3] = {cache->token_stride * 2, cache->head_stride * 2, cache->page_stride * 2};
-    const int b[4] = {64, box_keys, 1, 1};
-    if (!e4m3 && cache->pages > 0) {
-      if (int rc = make_tmap_4d(&tk, cache->k, p.dtype, d, st, b)) return rc;
-      if (int rc = make_tmap_4d(&tv, cache->v, p.dtype, d, st, b)) return rc;
+    const int64_t st8[3] = {cache->token_stride, cache->head_stride, cache->page_stride};
+    const int b[4] = {64, box_keys, 1, 1}, b8[4] = {128, box_keys, 1, 1};   // a row of codes is one span
+    if (cache->pages > 0) {
+      if (int rc = make_tmap_4d(&tk, cache->k, e4m3 ? FB200_U8 : p.dtype, d, e4m3 ? st8 : st, e4m3 ? b8 : b)) return rc;
+      if (int rc = make_tmap_4d(&tv, cache->v, e4m3 ? FB200_U8 : p.dtype, d, e4m3 ? st8 : st, e4m3 ? b8 : b)) return rc;
     }
   } else if (p.kv_rows > 0) {
     const int64_t d[4] = {p.dim, p.kv_rows, p.kv_heads, 1};
@@ -691,9 +841,9 @@ int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, boo
   if (int rc = device_status_word(&status)) return rc;
   const PagedCache view = cache != nullptr ? *cache : PagedCache{};
   auto launch = [&](auto kernel) -> int {
-    const size_t smem = ((tiles_small_bytes(spans, e4m3) + 1023) & ~1023u) + static_cast<size_t>(spans * kSpanBytes) * (2 + tiles_slots(spans, e4m3));
+    const size_t smem = ((tiles_small_bytes(spans, e4m3) + 1023) & ~1023u) + static_cast<size_t>(spans * kSpanBytes) * (2 + tiles_slots(spans, e4m3)) + (e4m3 ? kRawSlots * kSpanBytes : 0);
     FB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    kernel<<<static_cast<unsigned>(grid), tiles_threads(e4m3), smem, stream>>>(tq, tk, tv, p, view, tile_tokens, box_keys, status);
+    kernel<<<static_cast<unsigned>(grid), tiles_threads(e4m3), smem, stream>>>(tq, tk, tv, p, view, split, tile_tokens, box_keys, status);
     return FB200_OK;
   };
   auto pick = [&](auto type) -> int {
@@ -703,7 +853,12 @@ int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, boo
     return spans == 2 ? launch(attention_tiles_kernel<T, 2, true, false>) : launch(attention_tiles_kernel<T, 1, true, false>);
   };
   if (int rc = p.dtype == FB200_BF16 ? pick(__nv_bfloat16()) : pick(__half())) return rc;
-  return after_launch("attention_tiles_kernel");
+  if (int rc = after_launch("attention_tiles_kernel")) return rc;
+  if (split.parts == 1) return FB200_OK;
+  const int64_t joins = (static_cast<int64_t>(p.q_rows) * p.heads + 7) / 8;
+  if (p.dtype == FB200_BF16) attention_tiles_join_kernel<__nv_bfloat16><<<static_cast<unsigned>(joins), 256, 0, stream>>>(p, view, split, tile_tokens);
+  else attention_tiles_join_kernel<__half><<<static_cast<unsigned>(joins), 256, 0, stream>>>(p, view, split, tile_tokens);
+  return after_launch("attention_tiles_join_kernel");
 }
 
 }  // namespace fb200

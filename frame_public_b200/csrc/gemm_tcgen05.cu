@@ -877,7 +877,7 @@ int make_tmap_nchw_f32(CUtensorMap* map, const void* ptr, int64_t n, int64_t c, 
   return FB200_OK;
 }
 
-// Four dimensions of 16-bit elements (innermost contiguous, the other strides in bytes), boxes 128 bytes
+// Four dimensions of 16-bit elements or bytes (innermost contiguous, the other strides in bytes), boxes 128 bytes
 // wide with the 128-byte swizzle, zero fill outside.
 int make_tmap_4d(CUtensorMap* map, const void* ptr, int dtype, const int64_t (&dims)[4], const int64_t (&stride_bytes)[3],
                  const int (&box)[4]) {
@@ -890,7 +890,7 @@ int make_tmap_4d(CUtensorMap* map, const void* ptr, int dtype, const int64_t (&d
     gbox[i] = static_cast<cuuint32_t>(box[i]);
     if (i < 3) gstride[i] = static_cast<cuuint64_t>(stride_bytes[i]);
   }
-  CUresult r = fn(map, dtype == FB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+  CUresult r = fn(map, dtype == FB200_U8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : dtype == FB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                   const_cast<void*>(ptr), gdim, gstride, gbox, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {

@@ -101,20 +101,37 @@ __device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t pair) {
   return __half22float2(__half2(h));
 }
 
-// Codes in the high bytes of the two halves of x (the low bytes are ignored) as a pair of T.  bfloat16:
-// sign, exponent and mantissa move to their places, which is the value times 2^-120 (exponent bias 7
-// against 127; e4m3 denormals become bfloat16 denormals), and one exact product brings it back.  The code
-// 0x7F (NaN) is never written; it reads as 480 here.
-template <typename T> __device__ __forceinline__ uint32_t codes_to_pair(uint32_t x);
-template <> __device__ __forceinline__ uint32_t codes_to_pair<__nv_bfloat16>(uint32_t x) {
-  const uint32_t y = (x & 0x80008000u) | ((x & 0x7F007F00u) >> 4);
-  const uint32_t up = 0x7B807B80u;   // 2^120
-  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&up));
-  return *reinterpret_cast<const uint32_t*>(&r);
+// The low (high) two codes of a word as a pair of float16, exactly: one instruction at about one per cycle
+// and scheduler (measured).
+__device__ __forceinline__ uint32_t codes_low(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\t}" : "=r"(r) : "r"(w));
+  return r;
 }
-template <> __device__ __forceinline__ uint32_t codes_to_pair<__half>(uint32_t x) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(__byte_perm(x, 0, 0x4431)), __NV_E4M3);
-  return static_cast<uint32_t>(r.x) | (static_cast<uint32_t>(r.y) << 16);
+__device__ __forceinline__ uint32_t codes_high(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, y;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+// What the codes of a cache are multiplied with is float16 as well.  A bfloat16 query row is brought there by
+// the power of two that puts its largest magnitude into [2^14, 2^15): products with a power of two are exact,
+// and what falls below float16's smallest step (2^-24) is 2^-38 of that magnitude.  Returns the inverse's
+// exponent as a factor for the scores.
+__device__ __forceinline__ float query_lift(float amax, float& factor) {
+  const uint32_t e = __float_as_uint(amax) >> 23;   // biased; 0 and 255 (nothing, infinity, NaN) stay as they are
+  const bool plain = e >= 1u && e <= 254u;
+  // 2^(14 + 127 - e) from 2^-113 to 2^140: in two steps where one would leave fp32
+  const int up = plain ? 141 - static_cast<int>(e) : 0;
+  const int up1 = up > 120 ? 120 : up;
+  factor = __uint_as_float(static_cast<uint32_t>(127 + up1) << 23);
+  return __uint_as_float(static_cast<uint32_t>(127 - up1) << 23);
+}
+// A probability times its value's scale 2^e has to fit float16 too, so rows are normalised by the largest
+// 2^(score + e) instead of 2^score; e below this floor counts as the floor (rows of zeros have e = -126).
+constexpr int kScaleFloor = -60;
+__device__ __forceinline__ float scale_exponent(uint32_t b) {
+  const int e = static_cast<int>(b) - 127;
+  return static_cast<float>(e < kScaleFloor ? kScaleFloor : e);
 }
 
 // ---- host-side checks ----------------------------------------------------------------------------

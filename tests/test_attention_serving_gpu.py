@@ -108,6 +108,10 @@ PAGED = [
     (BF, 32, 4, 128, [33], [9000], 64, False, True, 1),                # few rows over a long cache
     (BF, 32, 4, 128, [1], [20000], 64, True, True, 1),
     (BF, 64, 1, 16, [1, 2], [50, 130], 16, False, True, 1),
+    (FH, 8, 1, 128, [40], [5000], 32, True, True, 1),                  # keys cut into parts, e4m3
+    (BF, 32, 2, 64, [40, 3], [3000, 2500], 16, True, False, 1),
+    (BF, 32, 2, 80, [2, 600], [4000, 1900], 64, False, True, 1),       # one block with parts, others without
+    (FH, 24, 2, 96, [3, 1], [2049, 1024], 16, True, True, 0),
 ]
 
 
@@ -236,6 +240,37 @@ def test_bad_pages_and_lengths_are_recorded_and_stay_inside():
     capi.attention_paged(p, cache, q.ptr, out.ptr, one.ptr, lens.ptr, pages.dev["table"].ptr, 3, work.ptr, size)
     capi.synchronize()
     assert capi.kernel_status(0) == 321
+
+
+def test_one_workspace_serves_calls_of_either_kind_and_a_short_max_kv():
+    """Decoding and split chunks in turn through one workspace; max_kv only shapes the schedule."""
+    dt, h, hk, d, page = BF, 16, 2, 128, 64
+    rng = np.random.default_rng(11)
+    lens = [3000, 2100]
+    pages = ref.Pages(rng, lens, page, hk, d, dt, False, True)
+    for s, n in enumerate(lens):
+        pages.put(s, 0, ref.store(rng.standard_normal((n, hk, d)), dt), ref.store(rng.standard_normal((n, hk, d)), dt))
+    cache, scale = pages.upload(), 1.0 / np.sqrt(d)
+    dlen = upload(np.array(lens, dtype=np.int32))
+    steps = [[1, 1], [20, 30], [1, 1], [2, 1], [64, 1], [1, 1]]
+    calls = []
+    for i, step in enumerate(steps):
+        cu = ref.offsets(step)
+        q = ref.store(rng.standard_normal((int(cu[-1]), h, d)), dt)
+        p = params(dt, h, hk, d, step, lens if i % 2 else [1100], len(q), 1, scale)
+        calls.append((step, cu, q, p, capi.attention_paged_workspace(p, cache)))
+    size = max(c[4] for c in calls)
+    work = upload(np.zeros(size, dtype=np.uint8))
+    for step, cu, q, p, _ in calls:
+        dq, dcu, out = upload(q), upload(cu), upload(np.full(q.shape, FILL, dtype=np.uint16))
+        lse = capi.DeviceBuffer(len(q) * h * 4)
+        capi.attention_paged(p, cache, dq.ptr, out.ptr, dcu.ptr, dlen.ptr, pages.dev["table"].ptr, pages.table.shape[1],
+                             work.ptr, size, lse=lse.ptr)
+        capi.synchronize()
+        assert capi.kernel_status(0) == 0
+        seqs = [tuple(pages.values(s, n)) for s, n in enumerate(lens)]
+        check_rows(out.download(np.uint16, q.shape), lse.download(np.float32, q.shape[:2]).astype(np.float64), q, cu, seqs,
+                   dt, d, np.float32(scale), 1)
 
 
 @pytest.mark.parametrize("coded", [False, True], ids=["same", "e4m3"])
