@@ -602,7 +602,8 @@ int launch_attention_decode(const ServingProblem& p, const PagedCache& cache, bo
   const bool big = p.dim > 64;
   const size_t smem = static_cast<size_t>(kDecodeWarps) * (kDecodeStages * 2 * (big ? 4096 : 2048) + 8 * (big ? 128 : 64) * 4 + 2 * kDecodeRows * 4);
   auto launch = [&](auto kernel) -> int {
-    FB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    static SmemOptIn opted;
+    if (int rc = opted.once(kernel, smem)) return rc;
     kernel<<<kDecodeMostCtas, kDecodeWarps * 32, smem, stream>>>(p, cache, static_cast<uint8_t*>(workspace), status);
     return FB200_OK;
   };

@@ -31,6 +31,28 @@ __device__ __forceinline__ void serving_lengths(const ServingProblem& p, const P
   }
 }
 
+// cudaFuncSetAttribute(MaxDynamicSharedMemorySize) once per kernel and device.  (The kernels of one launch
+// function have the same type, so a static in it is shared by all of them.)
+struct SmemOptIn {
+  static constexpr int kMost = 16;
+  std::atomic<const void*> who[kMost] = {};
+  std::atomic<uint64_t> done[kMost] = {};   // bit per device ordinal
+  template <typename K> int once(K kernel, size_t bytes) {
+    int device = 0, at = 0;
+    FB200_CUDA_OK(cudaGetDevice(&device));
+    const void* const f = reinterpret_cast<const void*>(kernel);
+    for (; at < kMost; ++at) {   // this kernel's place, or the first free one
+      const void* seen = nullptr;
+      if (who[at].load(std::memory_order_relaxed) == f || who[at].compare_exchange_strong(seen, f) || seen == f) break;
+    }
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if (at < kMost && (done[at].load(std::memory_order_acquire) & bit)) return FB200_OK;
+    FB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    if (at < kMost) done[at].fetch_or(bit, std::memory_order_release);
+    return FB200_OK;
+  }
+};
+
 // The front of every workspace: the decode kernel's counters, zero between calls; no other kernel touches it.
 constexpr size_t kServingCounterBytes = 4096;
 

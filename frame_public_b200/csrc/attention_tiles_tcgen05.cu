@@ -129,11 +129,17 @@ __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int 
     const int y = c * kTileKeys - lk + lq;   // blocks that end at or before token y see no more
     return blocks - max(0, min(y >= 0 ? y / tokens : 0, blocks - 1));
   };
+  int q0_mine = 0, lq_mine = 0, k0_mine = 0, lk_mine = 0;   // sequence `lane` stays in registers
+  if (lane < p.n_seqs) serving_lengths<PAGED>(p, cache, lane, q0_mine, lq_mine, k0_mine, lk_mine);
+  auto lengths = [&](int s, int& q0, int& lq, int& k0, int& lk) {
+    q0 = q0_mine, lq = lq_mine, k0 = k0_mine, lk = lk_mine;
+    if (s >= 32) serving_lengths<PAGED>(p, cache, s, q0, lq, k0, lk);
+  };
   auto total = [&](int c, int& longest) {
     int sum = 0, most = 0;
     for (int s = lane; s < p.n_seqs; s += 32) {
       int q0, lq, k0, lk;
-      serving_lengths<PAGED>(p, cache, s, q0, lq, k0, lk);
+      lengths(s, q0, lq, k0, lk);
       sum += above(lq, lk, c);
       most = max(most, lk);
       if (rank == 0 && c < 0 && lq > p.max_q) record_fault(status, kFaultBadLength);
@@ -156,7 +162,7 @@ __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int 
     const int s = s0 + lane;
     int q0 = 0, lq = 0, k0 = 0, lk = 0, n = 0, more = 0;
     if (s < p.n_seqs) {
-      serving_lengths<PAGED>(p, cache, s, q0, lq, k0, lk);
+      lengths(s, q0, lq, k0, lk);
       more = above(lq, lk, hi);
       n = above(lq, lk, hi - 1) - more;
     }
@@ -391,22 +397,26 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         if (!live) break;
         uint8_t* const to = base_ptr + (ring - base) + slot * kSlotBytes;
         const uint8_t* const raw = base_ptr + (raw_ring - base) + from * kSpanBytes;
-        auto convert = [&] {
-#pragma unroll 4
-          for (int i = 0; i < kTileKeys * kUnits / (kCodeWarps * 32); ++i) {
-            const int at = me + i * (kCodeWarps * 32), row = at / kUnits, unit = at % kUnits;
-            uint4 c = *reinterpret_cast<const uint4*>(raw + row * 128 + ((unit ^ (row & 7)) << 4));
-            if (key_tile + row >= item.lk) c = make_uint4(0, 0, 0, 0);
-            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+        // The rows a thread takes are multiples of 8 apart, so the swizzle is the same for all of them and
+        // every address is a constant away from the first.
+        constexpr int kApartRows = kCodeWarps * 32 / kUnits, kTakes = kTileKeys / kApartRows, kAhead = 8;
+        const int row0 = me / kUnits, unit = me % kUnits, left = item.lk - key_tile - row0;   // rows from row0 on that exist
+        const uint8_t* const in = raw + row0 * 128 + ((unit ^ (row0 & 7)) << 4);
+        uint8_t* const out = to + (unit >> 2) * kSpanBytes + row0 * 128;
+        const int out0 = (((unit & 3) * 2) ^ (row0 & 7)) << 4, out1 = (((unit & 3) * 2 + 1) ^ (row0 & 7)) << 4;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int chunk = ((unit & 3) * 2 + e) ^ (row & 7);
-              *reinterpret_cast<uint4*>(to + (unit >> 2) * kSpanBytes + row * 128 + chunk * 16) =
-                  make_uint4(codes_low(w[2 * e]), codes_high(w[2 * e]), codes_low(w[2 * e + 1]), codes_high(w[2 * e + 1]));
-            }
+        for (int i0 = 0; i0 < kTakes; i0 += kAhead) {
+          uint4 codes[kAhead];
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) codes[i] = *reinterpret_cast<const uint4*>(in + (i0 + i) * kApartRows * 128);
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            const uint4 w = (i0 + i) * kApartRows < left ? codes[i] : make_uint4(0, 0, 0, 0);
+            uint8_t* const at = out + (i0 + i) * kApartRows * 128;
+            *reinterpret_cast<uint4*>(at + out0) = make_uint4(codes_low(w.x), codes_high(w.x), codes_low(w.y), codes_high(w.y));
+            *reinterpret_cast<uint4*>(at + out1) = make_uint4(codes_low(w.z), codes_high(w.z), codes_low(w.w), codes_high(w.w));
           }
-        };
-        convert();
+        }
         if (!(n & 1)) {
           float* const sc = scales + ((n >> 1) % kScaleTiles) * 3 * kTileKeys;
 #pragma unroll
@@ -479,7 +489,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
       for (int j = 0; live && j < most; ++j) {
         const bool more = j + 1 < most;
-        if (more) live = mbar_wait_lanes(full + 8 * kp.slot, kp.phase, status, kFaultTilesKeys);
+        if (kApart && more) live = mbar_wait_lanes(full + 8 * kp.slot, kp.phase, status, kFaultTilesKeys);
         if (kApart && more && live) {
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
@@ -506,6 +516,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           if (live && j < tiles[s]) values(s, j);
+          if (!kApart && s == 0 && more) live = live && mbar_wait_lanes(full + 8 * kp.slot, kp.phase, status, kFaultTilesKeys);
           if (!kApart && live && j + 1 < tiles[s]) scores(s);
         }
         if (!live) break;
@@ -608,10 +619,13 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; E4M3 && i < kHalfKeys; i += 2) {   // of probability times value scale: see kScaleFloor
-        const float2 x = __fadd2_rn(make_float2(__uint_as_float(r[i >> 5][i & 31]), __uint_as_float(r[i >> 5][(i & 31) + 1])),
-                                    *reinterpret_cast<const float2*>(sc + 2 * kTileKeys + i));
-        top[(i >> 1) & 3] = fmaxf(top[(i >> 1) & 3], fmaxf(x.x, x.y));
+      for (int i = 0; E4M3 && i < kHalfKeys; i += 4) {   // of probability times value scale: see kScaleFloor
+        const float4 e4 = *reinterpret_cast<const float4*>(sc + 2 * kTileKeys + i);
+        const uint32_t* const x = &r[i >> 5][i & 31];
+        const float2 lo = __fadd2_rn(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), make_float2(e4.x, e4.y));
+        const float2 hi = __fadd2_rn(make_float2(__uint_as_float(x[2]), __uint_as_float(x[3])), make_float2(e4.z, e4.w));
+        top[(i >> 1) & 3] = fmaxf(top[(i >> 1) & 3], fmaxf(lo.x, lo.y));
+        top[((i >> 1) & 3) + 1] = fmaxf(top[((i >> 1) & 3) + 1], fmaxf(hi.x, hi.y));
       }
 #pragma unroll
       for (int i = 0; !E4M3 && i < kHalfKeys; i += 2) {
@@ -657,8 +671,10 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t out[16];
+        float4 v4;   // scales of V
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
+          if (E4M3 && !(e & 2)) v4 = *reinterpret_cast<const float4*>(sc + kTileKeys + i * 32 + e);
           float2 x = make_float2(__uint_as_float(r[i][e]), __uint_as_float(r[i][e + 1]));
           x = E4M3 ? __fadd2_rn(x, nm2) : __ffma2_rn(x, c2, nm2);
           if ((e & 15) == 14) {
@@ -668,7 +684,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             x.y = ex2(x.y);
           }
           sum = __fadd2_rn(sum, x);
-          if constexpr (E4M3) x = __fmul2_rn(x, *reinterpret_cast<const float2*>(sc + kTileKeys + i * 32 + e));
+          if constexpr (E4M3) x = __fmul2_rn(x, (e & 2) ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y));
           out[e >> 1] = pack_pair<M>(x.x, x.y);
         }
         tmem_st_32x32b_x16(t_p + i * 16, out);
@@ -842,7 +858,8 @@ int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, boo
   const PagedCache view = cache != nullptr ? *cache : PagedCache{};
   auto launch = [&](auto kernel) -> int {
     const size_t smem = ((tiles_small_bytes(spans, e4m3) + 1023) & ~1023u) + static_cast<size_t>(spans * kSpanBytes) * (2 + tiles_slots(spans, e4m3)) + (e4m3 ? kRawSlots * kSpanBytes : 0);
-    FB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    static SmemOptIn opted;
+    if (int rc = opted.once(kernel, smem)) return rc;
     kernel<<<static_cast<unsigned>(grid), tiles_threads(e4m3), smem, stream>>>(tq, tk, tv, p, view, split, tile_tokens, box_keys, status);
     return FB200_OK;
   };
