@@ -13,7 +13,7 @@
 //     head_dim 128: 128 KiB in flight per SM) and keeps its own running maximum, sum and O in registers; the
 //     four warps of a CTA meet only at the end of a pair's range, and the ring runs on across it.
 // e4m3 codes are turned into float16 operands in registers (exact, one conversion per two codes; bfloat16
-// takes five instructions, which bound the kernel: 130 us where this takes TIME_E4M3, 8 sequences over up to
+// takes five instructions, which bound the kernel: 130 us where this takes 79 us, 8 sequences over up to
 // 32000 keys); the scale of K multiplies the score, that of V the probability.  The contraction index of
 // Q K^T and the columns of O are permuted so that a thread reads 16 codes of one row at a time.
 #include <type_traits>

@@ -7,10 +7,13 @@
 // and code * 2^e is exact in bfloat16 when it is read.  A relative step of 2^-4 is all e4m3 has either
 // way; the scale only has to keep small numbers out of its denormals.
 // Read: code * 2^e, rounded once.
-// Both are bound by HBM: (2 + 1) bytes a number either way, 1/head_dim more for the scales.
+// Both are bound by HBM: (2 + 1) bytes a number either way, 1/head_dim more for the scales.  A lane group
+// (16 bytes a lane on the dense side) takes four heads of one token: the token's place, a binary search and two
+// dependent loads, is found once for eight vectors in flight (one head a group: TIME_BEFORE).
 #include "kv_cache.cuh"
 
 #include <climits>
+#include <type_traits>
 
 namespace fb200 {
 
@@ -76,77 +79,99 @@ struct DenseRows {
   int64_t k_token, k_head, v_token, v_head;   // in elements of two bytes
 };
 
-// One row's eight numbers of this lane into the cache.  The lanes of a row (LANES of them) hold all of
-// it; lanes at or past `lanes` hold nothing and only take part in the maximum.
-template <typename T, bool E4M3, int LANES>
-__device__ __forceinline__ void store_row(const uint4& raw, int lane, int lanes, uint8_t* codes, uint8_t* scale) {
-  if constexpr (!E4M3) {
-    if (lane < lanes) *reinterpret_cast<uint4*>(codes + lane * 16) = raw;
-  } else {
-    const T* x = reinterpret_cast<const T*>(&raw);
-    float f[8], amax = 0.0f;
-    bool finite = true;   // fmaxf drops a NaN, so it is looked for by itself
+// Largest magnitude of eight numbers as 16 bits.  Without their signs the bits are ordered like the
+// magnitudes, infinities above everything finite and NaNs above them.
+__device__ __forceinline__ uint32_t top_of(const uint4& x) {
+  const uint32_t m = 0x7FFF7FFFu;
+  const uint32_t t = __vmaxu2(__vmaxu2(x.x & m, x.y & m), __vmaxu2(x.z & m, x.w & m));
+  return max(t & 0xFFFFu, t >> 16);
+}
+template <typename T> __device__ __forceinline__ uint32_t f32_bits_of(uint32_t bits16) {
+  const uint16_t b = static_cast<uint16_t>(bits16);
+  return __float_as_uint(to_f32(*reinterpret_cast<const T*>(&b)));
+}
+// Eight numbers of a row whose largest magnitude is `top` (16 bits), as codes.
+template <typename T> __device__ __forceinline__ uint2 encode8(const uint4& raw, uint32_t byte) {
+  if (byte == 255u) return make_uint2(0u, 0u);   // not finite
+  // 2^-e = 2^(127 - byte): exponent field 254 - byte, above 0 (amax < 2^128 gives at most byte 247)
+  const float inv = __uint_as_float((254u - byte) << 23);
+  const T* x = reinterpret_cast<const T*>(&raw);
+  uint32_t out[2] = {0u, 0u};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[i] = to_f32(x[i]);
-      amax = fmaxf(amax, fabsf(f[i]));
-      finite = finite && fabsf(f[i]) < INFINITY;
-    }
-    uint32_t top = finite ? __float_as_uint(amax) : 0x7F800000u;   // non-negative: ordered as integers
-#pragma unroll
-    for (int d = LANES / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d, LANES));
-    const uint32_t byte = scale_byte_of(top);
-    // 2^-e = 2^(127 - byte): exponent field 254 - byte, from 0 (byte 254, never met: amax < 2^128) up
-    const float inv = byte == 255u ? 0.0f : __uint_as_float((254u - byte) << 23);
-    uint32_t out[2] = {0u, 0u};
-    if (byte != 255u) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t pair = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i] * inv, f[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-        out[i >> 1] |= pair << ((i & 1) * 16);
-      }
-    }
-    if (lane < lanes) *reinterpret_cast<uint2*>(codes + lane * 8) = make_uint2(out[0], out[1]);
-    if (lane == 0) *scale = static_cast<uint8_t>(byte);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t pair = __nv_cvt_float2_to_fp8x2(make_float2(to_f32(x[2 * i]) * inv, to_f32(x[2 * i + 1]) * inv), __NV_SATFINITE, __NV_E4M3);
+    out[i >> 1] |= pair << ((i & 1) * 16);
   }
+  return make_uint2(out[0], out[1]);
 }
 
-template <typename T, bool E4M3, int LANES>
+// The token and the heads a lane group works on.
+struct Unit {
+  int row, head, heads;   // heads: how many from `head` on, 0 past the end
+};
+template <int LANES, int HEADS> __device__ __forceinline__ Unit unit_of(int rows, int heads) {
+  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / LANES;
+  const int per_row = (heads + HEADS - 1) / HEADS;
+  if (unit >= static_cast<int64_t>(rows) * per_row) return {0, 0, 0};
+  const int row = static_cast<int>(unit / per_row), head = static_cast<int>(unit - static_cast<int64_t>(row) * per_row) * HEADS;
+  return {row, head, min(HEADS, heads - head)};
+}
+// Page of token `pos` of sequence seq, or -1 (recorded) if it has no place.
+__device__ __forceinline__ int place_of(const PagedCache& cache, int seq, int64_t pos, int* status) {
+  if (pos < 0 || (pos >> cache.page_shift) >= cache.table_stride) {
+    record_fault(status, kFaultBadLength);
+    return -1;
+  }
+  const int page = cache.table[seq * cache.table_stride + (pos >> cache.page_shift)];
+  if (static_cast<uint32_t>(page) < static_cast<uint32_t>(cache.pages)) return page;
+  record_fault(status, kFaultBadPage);
+  return -1;
+}
+
+template <typename T, bool E4M3, int LANES, int HEADS>
 __global__ void __launch_bounds__(256) kv_cache_write_kernel(PagedCache cache, DenseRows in, const int32_t* __restrict__ cu_q,
                                                              const int32_t* __restrict__ kv_len, int n_seqs, int rows,
                                                              int heads, int lanes, int* status) {
-  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / LANES;
   const int lane = threadIdx.x & (LANES - 1);
-  const bool there = unit < static_cast<int64_t>(rows) * heads;
-  const int row = there ? static_cast<int>(unit / heads) : 0, head = there ? static_cast<int>(unit - static_cast<int64_t>(row) * heads) : 0;
+  const Unit u = unit_of<LANES, HEADS>(rows, heads);
   // the loads do not wait for the lookups of where the row goes
-  uint4 k = make_uint4(0, 0, 0, 0), v = k;
-  if (there && lane < lanes) {
-    k = __ldg(reinterpret_cast<const uint4*>(in.k + 2 * (row * in.k_token + head * in.k_head)) + lane);
-    v = __ldg(reinterpret_cast<const uint4*>(in.v + 2 * (row * in.v_token + head * in.v_head)) + lane);
-  }
-  const int seq = there ? sequence_of_row(cu_q, n_seqs, row) : -1;
-  int page = -1, token = 0;
-  if (seq >= 0) {
-    const int64_t pos = static_cast<int64_t>(kv_len[seq]) - cu_q[seq + 1] + row;
-    if (pos < 0 || (pos >> cache.page_shift) >= cache.table_stride) {
-      record_fault(status, kFaultBadLength);
-    } else {
-      token = static_cast<int>(pos);
-      page = cache.table[seq * cache.table_stride + (pos >> cache.page_shift)];
-      if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(cache.pages)) {
-        record_fault(status, kFaultBadPage);
-        page = -1;
-      }
+  uint4 k[HEADS], v[HEADS];
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i) {
+    k[i] = v[i] = make_uint4(0, 0, 0, 0);
+    if (i < u.heads && lane < lanes) {
+      k[i] = __ldg(reinterpret_cast<const uint4*>(in.k + 2 * (u.row * in.k_token + (u.head + i) * in.k_head)) + lane);
+      v[i] = __ldg(reinterpret_cast<const uint4*>(in.v + 2 * (u.row * in.v_token + (u.head + i) * in.v_head)) + lane);
     }
   }
-  const bool store = page >= 0;
-  const int mine = store ? lanes : 0, lead = store ? lane : -1;   // lead: lane 0 of a stored row writes the scale
-  const int64_t at = store ? token_offset(cache, page, token, head) : 0;
-  const int64_t sat = store && E4M3 ? scale_offset(cache, page, token, head) : 0;
+  const int seq = u.heads > 0 ? sequence_of_row(cu_q, n_seqs, u.row) : -1;
+  const int64_t pos = seq >= 0 ? static_cast<int64_t>(kv_len[seq]) - cu_q[seq + 1] + u.row : 0;
+  const int page = seq >= 0 ? place_of(cache, seq, pos, status) : -1;
   constexpr int kBytes = E4M3 ? 1 : 2;
-  store_row<T, E4M3, LANES>(k, lead < 0 ? LANES : lead, mine, cache.k + at * kBytes, cache.k_scale + sat);
-  store_row<T, E4M3, LANES>(v, lead < 0 ? LANES : lead, mine, cache.v + at * kBytes, cache.v_scale + sat);
+  const int64_t at = page >= 0 ? token_offset(cache, page, static_cast<int>(pos), u.head) * kBytes : 0;
+  const int64_t sat = page >= 0 && E4M3 ? scale_offset(cache, page, static_cast<int>(pos), u.head) : 0;
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i) {
+    const bool store = page >= 0 && i < u.heads && lane < lanes;   // the others only take part in the maximum
+    const int64_t to = at + i * cache.head_stride * kBytes;
+    if constexpr (E4M3) {
+      uint32_t top = top_of(k[i]) | top_of(v[i]) << 16;   // both rows' maxima in one word
+#pragma unroll
+      for (int d = LANES / 2; d > 0; d >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d, LANES));
+      const uint32_t kb = scale_byte_of(f32_bits_of<T>(top & 0xFFFFu)), vb = scale_byte_of(f32_bits_of<T>(top >> 16));
+      if (store) {
+        *reinterpret_cast<uint2*>(cache.k + to + lane * 8) = encode8<T>(k[i], kb);
+        *reinterpret_cast<uint2*>(cache.v + to + lane * 8) = encode8<T>(v[i], vb);
+        if (lane == 0) {
+          cache.k_scale[sat + i * cache.scale_head_stride] = static_cast<uint8_t>(kb);
+          cache.v_scale[sat + i * cache.scale_head_stride] = static_cast<uint8_t>(vb);
+        }
+      }
+    } else if (store) {
+      *reinterpret_cast<uint4*>(cache.k + to + lane * 16) = k[i];
+      *reinterpret_cast<uint4*>(cache.v + to + lane * 16) = v[i];
+    }
+  }
 }
 
 // Eight codes times the row's scale, rounded once to T.
@@ -161,40 +186,46 @@ template <typename T> __device__ __forceinline__ uint4 decode8(uint2 codes, floa
   return *reinterpret_cast<const uint4*>(out);
 }
 
-template <typename T, bool E4M3, int LANES>
+template <typename T, bool E4M3, int LANES, int HEADS>
 __global__ void __launch_bounds__(256) kv_cache_read_kernel(PagedCache cache, DenseRows out, const int32_t* __restrict__ cu_kv,
                                                             int n_seqs, int rows, int heads, int lanes, int* status) {
-  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / LANES;
   const int lane = threadIdx.x & (LANES - 1);
-  if (unit >= static_cast<int64_t>(rows) * heads || lane >= lanes) return;
-  const int row = static_cast<int>(unit / heads), head = static_cast<int>(unit - static_cast<int64_t>(row) * heads);
-  const int seq = sequence_of_row(cu_kv, n_seqs, row);
+  const Unit u = unit_of<LANES, HEADS>(rows, heads);
+  if (u.heads == 0 || lane >= lanes) return;
+  const int seq = sequence_of_row(cu_kv, n_seqs, u.row);
   if (seq < 0) return;
-  const int64_t pos = static_cast<int64_t>(row) - cu_kv[seq];
-  if (pos < 0 || (pos >> cache.page_shift) >= cache.table_stride) {
-    record_fault(status, kFaultBadLength);
-    return;
+  const int64_t pos = static_cast<int64_t>(u.row) - cu_kv[seq];
+  const int page = place_of(cache, seq, pos, status);
+  if (page < 0) return;
+  using Raw = typename std::conditional<E4M3, uint2, uint4>::type;   // eight numbers
+  const int64_t at = token_offset(cache, page, static_cast<int>(pos), u.head) * (E4M3 ? 1 : 2) + lane * sizeof(Raw);
+  const int64_t step = cache.head_stride * (E4M3 ? 1 : 2);
+  Raw k[HEADS], v[HEADS];
+  uint32_t ks[HEADS], vs[HEADS];
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i) {
+    if (i >= u.heads) break;
+    k[i] = *reinterpret_cast<const Raw*>(cache.k + at + i * step);
+    v[i] = *reinterpret_cast<const Raw*>(cache.v + at + i * step);
+    if constexpr (E4M3) {
+      const int64_t sat = scale_offset(cache, page, static_cast<int>(pos), u.head + i);
+      ks[i] = cache.k_scale[sat];
+      vs[i] = cache.v_scale[sat];
+    }
   }
-  const int token = static_cast<int>(pos);
-  const int page = cache.table[seq * cache.table_stride + (pos >> cache.page_shift)];
-  if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(cache.pages)) {
-    record_fault(status, kFaultBadPage);
-    return;
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i) {
+    if (i >= u.heads) break;
+    uint4* const to_k = reinterpret_cast<uint4*>(out.k + 2 * (u.row * out.k_token + (u.head + i) * out.k_head)) + lane;
+    uint4* const to_v = reinterpret_cast<uint4*>(out.v + 2 * (u.row * out.v_token + (u.head + i) * out.v_head)) + lane;
+    if constexpr (E4M3) {
+      *to_k = decode8<T>(k[i], scale_of_byte(ks[i]));
+      *to_v = decode8<T>(v[i], scale_of_byte(vs[i]));
+    } else {
+      *to_k = k[i];
+      *to_v = v[i];
+    }
   }
-  const int64_t at = token_offset(cache, page, token, head);
-  uint4 k, v;
-  if constexpr (E4M3) {
-    const int64_t sat = scale_offset(cache, page, token, head);
-    const uint2 kc = *reinterpret_cast<const uint2*>(cache.k + at + lane * 8);
-    const uint2 vc = *reinterpret_cast<const uint2*>(cache.v + at + lane * 8);
-    k = decode8<T>(kc, scale_of_byte(cache.k_scale[sat]));
-    v = decode8<T>(vc, scale_of_byte(cache.v_scale[sat]));
-  } else {
-    k = *reinterpret_cast<const uint4*>(cache.k + at * 2 + lane * 16);
-    v = *reinterpret_cast<const uint4*>(cache.v + at * 2 + lane * 16);
-  }
-  *(reinterpret_cast<uint4*>(out.k + 2 * (row * out.k_token + head * out.k_head)) + lane) = k;
-  *(reinterpret_cast<uint4*>(out.v + 2 * (row * out.v_token + head * out.v_head)) + lane) = v;
 }
 
 static int check_rows(const char* what, const fb200_kv_cache* cache, const void* k, int64_t kt, int64_t kh, const void* v,
@@ -216,29 +247,32 @@ static int check_rows(const char* what, const fb200_kv_cache* cache, const void*
   return FB200_OK;
 }
 
+// Lanes per row: 8 cover head_dim 64, 16 cover 128 (one 16-byte vector of the dense side each).  Four heads a
+// group when that still leaves two groups' worth of work for every thread slot of the GPU (16 prompts of up to
+// 4000 tokens, 8 heads: write 44 -> 35 us), one where the call is too small for it (32 single tokens: 3.1 us
+// against 4.7).
+template <typename Go>
+static void dispatch_rows(const fb200_kv_cache* cache, int64_t rows, int dtype, Go go) {
+  const int lanes = static_cast<int>(cache->head_dim / 8), group = lanes <= 8 ? 8 : 16;
+  const bool wide = rows * cache->kv_heads * group >= int64_t(2) * kNumSMs * 2048 && cache->kv_heads >= 4;
+  const int64_t per_row = wide ? (cache->kv_heads + 3) / 4 : cache->kv_heads;
+  const unsigned grid = static_cast<unsigned>((rows * per_row * group + 255) / 256);
+  auto heads = [&](auto type, auto e4m3, auto width) {
+    if (wide) go(type, e4m3, width, std::integral_constant<int, 4>(), grid, lanes);
+    else go(type, e4m3, width, std::integral_constant<int, 1>(), grid, lanes);
+  };
+  auto width = [&](auto type, auto e4m3) {
+    if (group == 8) heads(type, e4m3, std::integral_constant<int, 8>());
+    else heads(type, e4m3, std::integral_constant<int, 16>());
+  };
+  if (cache->dtype != FB200_U8) width(__nv_bfloat16(), std::false_type());   // 16 bits move as they are
+  else if (dtype == FB200_BF16) width(__nv_bfloat16(), std::true_type());
+  else width(__half(), std::true_type());
+}
+
 }  // namespace fb200
 
 using namespace fb200;
-
-// Lanes per row: 8 cover head_dim 64, 16 cover 128 (one 16-byte vector of the dense side each).
-#define FB200_KV_DISPATCH(KERNEL, ...)                                                                    \
-  do {                                                                                                    \
-    const int lanes = static_cast<int>(cache->head_dim / 8), group = lanes <= 8 ? 8 : 16;                 \
-    const unsigned grid = static_cast<unsigned>((rows * cache->kv_heads * group + 255) / 256);            \
-    const int heads = static_cast<int>(cache->kv_heads);                                                  \
-    cudaStream_t s = as_stream(stream);                                                                   \
-    auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(__VA_ARGS__, heads, lanes, status); };       \
-    const bool bf = dtype == FB200_BF16, e4m3 = cache->dtype == FB200_U8;                                 \
-    if (group == 8) {                                                                                     \
-      if (!e4m3) go(KERNEL<__nv_bfloat16, false, 8>);                                                     \
-      else if (bf) go(KERNEL<__nv_bfloat16, true, 8>);                                                    \
-      else go(KERNEL<__half, true, 8>);                                                                   \
-    } else {                                                                                              \
-      if (!e4m3) go(KERNEL<__nv_bfloat16, false, 16>);                                                    \
-      else if (bf) go(KERNEL<__nv_bfloat16, true, 16>);                                                   \
-      else go(KERNEL<__half, true, 16>);                                                                  \
-    }                                                                                                     \
-  } while (0)
 
 extern "C" int fb200_kv_cache_write(const fb200_kv_cache* cache, const void* k, int64_t k_token_stride, int64_t k_head_stride,
                                     const void* v, int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_q,
@@ -256,7 +290,11 @@ extern "C" int fb200_kv_cache_write(const fb200_kv_cache* cache, const void* k, 
   if (int rc = device_status_word(&status)) return rc;
   const DenseRows in{static_cast<uint8_t*>(const_cast<void*>(k)), static_cast<uint8_t*>(const_cast<void*>(v)),
                      k_token_stride, k_head_stride, v_token_stride, v_head_stride};
-  FB200_KV_DISPATCH(kv_cache_write_kernel, c, in, cu_q, kv_len, static_cast<int>(n_seqs), static_cast<int>(rows));
+  dispatch_rows(cache, rows, dtype, [&](auto type, auto e4m3, auto width, auto heads, unsigned grid, int lanes) {
+    kv_cache_write_kernel<decltype(type), decltype(e4m3)::value, decltype(width)::value, decltype(heads)::value>
+        <<<grid, 256, 0, as_stream(stream)>>>(c, in, cu_q, kv_len, static_cast<int>(n_seqs), static_cast<int>(rows),
+                                              static_cast<int>(cache->kv_heads), lanes, status);
+  });
   return after_launch("kv_cache_write_kernel");
 }
 
@@ -275,6 +313,10 @@ extern "C" int fb200_kv_cache_read(const fb200_kv_cache* cache, void* k, int64_t
   if (int rc = device_status_word(&status)) return rc;
   const DenseRows out{static_cast<uint8_t*>(k), static_cast<uint8_t*>(v), k_token_stride, k_head_stride, v_token_stride,
                       v_head_stride};
-  FB200_KV_DISPATCH(kv_cache_read_kernel, c, out, cu_kv, static_cast<int>(n_seqs), static_cast<int>(rows));
+  dispatch_rows(cache, rows, dtype, [&](auto type, auto e4m3, auto width, auto heads, unsigned grid, int lanes) {
+    kv_cache_read_kernel<decltype(type), decltype(e4m3)::value, decltype(width)::value, decltype(heads)::value>
+        <<<grid, 256, 0, as_stream(stream)>>>(c, out, cu_kv, static_cast<int>(n_seqs), static_cast<int>(rows),
+                                              static_cast<int>(cache->kv_heads), lanes, status);
+  });
   return after_launch("kv_cache_read_kernel");
 }
