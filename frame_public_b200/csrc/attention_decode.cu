@@ -27,6 +27,7 @@ int device_status_word(int** dev_ptr);
 constexpr int kDecodeWarps = 4;
 constexpr int kDecodeStages = 3;
 constexpr int kDecodeCtasPerSm = 2;
+constexpr int kDecodeJoinRows = 4;
 constexpr int kDecodeMostCtas = kNumSMs * kDecodeCtasPerSm;
 constexpr int kDecodeRows = 16;
 constexpr int kDecodeSlabBytes = 4096;      // K or V of one slab at head_dim 65..128; half below
@@ -110,8 +111,9 @@ __device__ __forceinline__ void cursor_next(const ServingProblem& p, const Paged
   at.left -= at.end;
 }
 
-// BIG: head_dim 65..128, else up to 64.
-template <typename T, bool BIG, bool E4M3>
+// BIG: head_dim 65..128, else up to 64.  HALVES: 1 when a kv head has at most 8 rows (the tile's upper half
+// stays empty and costs no softmax), else 2.
+template <typename T, bool BIG, bool E4M3, int HALVES>
 __global__ void __launch_bounds__(kDecodeWarps * 32, kDecodeCtasPerSm)
 attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t* workspace, int* status) {
   constexpr int kSlab = E4M3 ? 32 : 16;                    // keys of a warp's slab
@@ -129,11 +131,26 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g4 = lane >> 2, t = lane & 3;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (kDecodeStages * 2 * kHalf);
-  float* const join_o = reinterpret_cast<float*>(smem + kDecodeWarps * kDecodeStages * 2 * kHalf);   // [warps][8][kDim]
-  float* const join_m = join_o + kDecodeWarps * 8 * kDim;                                            // [warps][16]
+  float* const join_o = reinterpret_cast<float*>(smem + kDecodeWarps * kDecodeStages * 2 * kHalf);   // [warps][kDecodeJoinRows][kDim]
+  float* const join_m = join_o + kDecodeWarps * kDecodeJoinRows * kDim;                                            // [warps][16]
   float* const join_l = join_m + kDecodeWarps * kDecodeRows;
   __shared__ int last_flag;
   const int units = p.dim * (E4M3 ? 1 : 2) / 16, steps = p.dim / 16;
+
+  // Where a lane reads in a slab of codes; rows are constants away (the swizzles depend on the lane alone).
+  uint32_t lane_k[2] = {0, 0}, lane_v = 0;
+  if constexpr (E4M3) {
+    const int row_swap = BIG ? (g4 & 1) << 2 : 0;
+    lane_k[0] = g4 * kRowBytes + ((t ^ row_swap) << 4);
+    lane_k[1] = g4 * kRowBytes + (((4 + t) ^ row_swap) << 4);
+    lane_v = t * 2 * kRowBytes + (BIG ? (g4 ^ (t * 2)) << 4 : (((g4 >> 1) ^ t) << 4) + (g4 & 1) * 8);
+    if (units < kUnits) {   // what no copy fills reads as zeros
+      for (int i = lane; i < kDecodeStages * 2 * kHalf / 16; i += 32) {
+        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + i * 16), "r"(0) : "memory");
+      }
+      __syncwarp();
+    }
+  }
 
   // ---- this CTA's range -----------------------------------------------------------------------------
   int64_t total = 0;
@@ -259,17 +276,16 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
     }
     const int rows = lq * p.group, head = take.head, first_tile = take.tile, end_tile = take.end;
     const int pair_n = take.tiles;
-    uint32_t q[kSteps][4];
-    int limit[2];
+    uint32_t q[kSteps][4] = {};
+    int limit[2] = {0, 0};
     float lift[2] = {c, c};   // of the scores, to the exponent's units
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int half = 0; half < HALVES; ++half) {
       const int r = g4 + half * 8, i = r / p.group;
       limit[half] = r < rows ? (p.causal ? min(lk, i + shift + 1) : lk) : 0;
       const uint8_t* src = p.q + 2 * ((q0 + i) * p.q_token + (head * p.group + r - i * p.group) * p.q_head);
 #pragma unroll
       for (int ks = 0; ks < kSteps; ++ks) {
-        q[ks][half] = q[ks][half + 2] = 0;
         if constexpr (E4M3) {
           const int d = (ks >> 2) * 64 + t * 16 + (ks & 3) * 4;   // four numbers in a row: k = 2t, 2t+1, 2t+8, 2t+9
           if (r < rows && d < p.dim) {
@@ -338,12 +354,9 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
       if constexpr (E4M3) {
 #pragma unroll
         for (int n = 0; n < kKeyTiles; ++n) {
-          const int row = n * 8 + g4;
 #pragma unroll
           for (int i = 0; i < kSteps / 4; ++i) {
-            const int unit = i * 4 + t;
-            uint4 x = lds128(ks_at + row * kRowBytes + ((unit ^ (BIG ? (row & 1) << 2 : 0)) << 4));
-            if (unit >= units) x = make_uint4(0, 0, 0, 0);
+            const uint4 x = lds128(ks_at + lane_k[i] + n * 8 * kRowBytes);
             const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -380,7 +393,7 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
             weight = __shfl_sync(0xffffffffu, v_exp, at);
           }
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+          for (int half = 0; half < HALVES; ++half) {
             float x = s[n][half * 2 + e] * lift[half];
             if constexpr (E4M3) x *= f;
             if (edge && key >= limit[half]) x = -INFINITY;
@@ -390,15 +403,15 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
         }
       }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int half = 0; half < HALVES; ++half) {
         top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
         top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
       }
       // O follows a row's maximum once it grew by more than 2^8 (or for the first time).
-      if (__any_sync(0xffffffffu, top[0] - m[0] > 8.0f || top[1] - m[1] > 8.0f)) {
-        float f[2];
+      if (__any_sync(0xffffffffu, top[0] - m[0] > 8.0f || (HALVES == 2 && top[1] - m[1] > 8.0f))) {
+        float f[2] = {1.0f, 1.0f};
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < HALVES; ++half) {
           const float next = fmaxf(m[half], top[half]);
           f[half] = next == -INFINITY ? 1.0f : exp2_fast(m[half] - next);
           m[half] = next;
@@ -408,20 +421,26 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
         for (int j = 0; j < kCols; ++j) {
           o[j][0] *= f[0];
           o[j][1] *= f[0];
-          o[j][2] *= f[1];
-          o[j][3] *= f[1];
+          if (HALVES == 2) {
+            o[j][2] *= f[1];
+            o[j][3] *= f[1];
+          }
         }
       }
       const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-      uint32_t pa[kKeyTiles / 2][4];   // P as A operands of 16 keys each
+      uint32_t pa[kKeyTiles / 2][4] = {};   // P as A operands of 16 keys each
 #pragma unroll
       for (int n = 0; n < kKeyTiles; ++n) {
+        float v0 = 1.0f, v1 = 1.0f;
+        if constexpr (E4M3) {
+          v0 = __shfl_sync(0xffffffffu, v_factor, n * 8 + t * 2);
+          v1 = __shfl_sync(0xffffffffu, v_factor, n * 8 + t * 2 + 1);
+        }
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < HALVES; ++half) {
           float e0 = exp2_fast(s[n][half * 2] - base[half]), e1 = exp2_fast(s[n][half * 2 + 1] - base[half]);
           l[half] += e0 + e1;
           if constexpr (E4M3) {
-            const float v0 = __shfl_sync(0xffffffffu, v_factor, n * 8 + t * 2), v1 = __shfl_sync(0xffffffffu, v_factor, n * 8 + t * 2 + 1);
             const int key = key0 + n * 8 + t * 2;
             // a masked key's scale may be NaN
             e0 = edge && key >= limit[half] ? 0.0f : e0 * v0;
@@ -439,15 +458,12 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
       // ---- O += P V ----------------------------------------------------------------------------------
       if constexpr (E4M3) {
         constexpr int kWords = kCols / 4;   // a thread's codes of one key: columns d = g4 * kCols + 0 .. kCols - 1
-        const int unit = BIG ? g4 : g4 >> 1, inside = BIG ? 0 : (g4 & 1) * 8;
-        const bool there = g4 * kCols < p.dim;
 #pragma unroll
         for (int k = 0; k < kKeyTiles / 2; ++k) {
           uint32_t w[4][kWords];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int row = k * 16 + t * 2 + (i & 1) + (i >> 1) * 8;
-            const uint32_t at = vs_at + row * kRowBytes + ((unit ^ (BIG ? row & 6 : (row >> 1) & 3)) << 4) + inside;
+            const uint32_t at = vs_at + lane_v + (k * 16 + (i & 1) + (i >> 1) * 8) * kRowBytes;
             if constexpr (BIG) {
               const uint4 x = lds128(at);
               w[i][0] = x.x, w[i][1] = x.y, w[i][2] = x.z, w[i][3] = x.w;
@@ -455,8 +471,6 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
               const uint2 x = lds64(at);
               w[i][0] = x.x, w[i][1] = x.y;
             }
-#pragma unroll
-            for (int j = 0; j < kWords; ++j) w[i][j] = there ? w[i][j] : 0u;
           }
 #pragma unroll
           for (int j = 0; j < kCols; j += 2) {   // bytes j, j + 1 of the one key and of the other, in turn
@@ -485,7 +499,7 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
 
     // ---- the four warps' shares meet ------------------------------------------------------------------
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int half = 0; half < HALVES; ++half) {
       l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
       l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
       if (t == 0) {
@@ -513,12 +527,13 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
         p.lse[static_cast<int64_t>(q0 + i) * p.heads + h] = lr == 0.0f ? -INFINITY : mr * 0.6931471805599453f + logf(lr);
       }
     };
-    for (int r0 = 0; r0 < rows; r0 += 8) {
+    for (int r0 = 0; r0 < rows; r0 += kDecodeJoinRows) {
       const int half = r0 >> 3;
       if (r0 > 0) __syncthreads();
-      float* const mine = join_o + (warp * 8 + g4) * kDim;
+      float* const mine = join_o + (warp * kDecodeJoinRows + (g4 & (kDecodeJoinRows - 1))) * kDim;
+      const bool turn = (g4 & ~(kDecodeJoinRows - 1)) == (r0 & 7);
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) {
+      for (int j = 0; turn && j < kCols; ++j) {
         const float x = half ? o[j][2] : o[j][0], y = half ? o[j][3] : o[j][1];
         if constexpr (E4M3) {
           mine[t * 2 * kCols + j] = x;
@@ -528,7 +543,7 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
         }
       }
       __syncthreads();
-      for (int i = tid; i < 8 * quads; i += kDecodeWarps * 32) {
+      for (int i = tid; i < kDecodeJoinRows * quads; i += kDecodeWarps * 32) {
         const int rr = i / quads, r = r0 + rr, d = (i - rr * quads) * 4;
         if (r >= rows) break;
         float mr = -INFINITY, lr = 0.0f;
@@ -536,7 +551,7 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
         float4 sum = make_float4(0, 0, 0, 0);
         for (int w = 0; w < kDecodeWarps; ++w) {
           const float mw = join_m[w * kDecodeRows + r], f = mw == -INFINITY ? 0.0f : exp2_fast(mw - mr);
-          const float4 x = *reinterpret_cast<const float4*>(join_o + (w * 8 + rr) * kDim + d);
+          const float4 x = *reinterpret_cast<const float4*>(join_o + (w * kDecodeJoinRows + rr) * kDim + d);
           lr += f * join_l[w * kDecodeRows + r];
           sum.x += f * x.x;
           sum.y += f * x.y;
@@ -619,22 +634,21 @@ int launch_attention_decode(const ServingProblem& p, const PagedCache& cache, bo
   int* status = nullptr;
   if (int rc = device_status_word(&status)) return rc;
   const bool big = p.dim > 64;
-  const size_t smem = static_cast<size_t>(kDecodeWarps) * (kDecodeStages * 2 * (big ? 4096 : 2048) + 8 * (big ? 128 : 64) * 4 + 2 * kDecodeRows * 4);
+  const size_t smem = static_cast<size_t>(kDecodeWarps) * (kDecodeStages * 2 * (big ? 4096 : 2048) + kDecodeJoinRows * (big ? 128 : 64) * 4 + 2 * kDecodeRows * 4);
   auto launch = [&](auto kernel) -> int {
     static SmemOptIn opted;
     if (int rc = opted.once(kernel, smem)) return rc;
     kernel<<<kDecodeMostCtas, kDecodeWarps * 32, smem, stream>>>(p, cache, static_cast<uint8_t*>(workspace), status);
     return FB200_OK;
   };
-  const bool bf = p.dtype == FB200_BF16;
-  int rc;
-  if (big) {
-    if (e4m3) rc = bf ? launch(attention_decode_kernel<__nv_bfloat16, true, true>) : launch(attention_decode_kernel<__half, true, true>);
-    else rc = bf ? launch(attention_decode_kernel<__nv_bfloat16, true, false>) : launch(attention_decode_kernel<__half, true, false>);
-  } else {
-    if (e4m3) rc = bf ? launch(attention_decode_kernel<__nv_bfloat16, false, true>) : launch(attention_decode_kernel<__half, false, true>);
-    else rc = bf ? launch(attention_decode_kernel<__nv_bfloat16, false, false>) : launch(attention_decode_kernel<__half, false, false>);
-  }
+  auto rows = [&](auto type, auto big_dim, auto codes) -> int {
+    using T = decltype(type);
+    constexpr bool kBig = decltype(big_dim)::value, kCodes = decltype(codes)::value;
+    return p.max_q * p.group <= 8 ? launch(attention_decode_kernel<T, kBig, kCodes, 1>) : launch(attention_decode_kernel<T, kBig, kCodes, 2>);
+  };
+  auto dims = [&](auto type, auto codes) -> int { return big ? rows(type, std::true_type(), codes) : rows(type, std::false_type(), codes); };
+  auto kind = [&](auto type) -> int { return e4m3 ? dims(type, std::true_type()) : dims(type, std::false_type()); };
+  const int rc = p.dtype == FB200_BF16 ? kind(__nv_bfloat16()) : kind(__half());
   if (rc != FB200_OK) return rc;
   return after_launch("attention_decode_kernel");
 }
