@@ -127,10 +127,12 @@ __device__ __forceinline__ float query_lift(float amax, float& factor) {
   return __uint_as_float(static_cast<uint32_t>(127 - up1) << 23);
 }
 // A probability times its value's scale 2^e has to fit float16 too, so rows are normalised by the largest
-// 2^(score + e) instead of 2^score; e below this floor counts as the floor (rows of zeros have e = -126).
+// 2^(score + e) instead of 2^score.  e below a floor counts as the floor (rows of zeros have e = -126), and so
+// does that of a row that is not finite, which makes NaN of the result through its scale.  The row sum is then
+// down to 2^-e of its largest term: above e = 100 (values past 10^32) terms 2^-26 of it start to be lost.
 constexpr int kScaleFloor = -60;
 __device__ __forceinline__ float scale_exponent(uint32_t b) {
-  const int e = static_cast<int>(b) - 127;
+  const int e = b == 255u ? kScaleFloor : static_cast<int>(b) - 127;
   return static_cast<float>(e < kScaleFloor ? kScaleFloor : e);
 }
 

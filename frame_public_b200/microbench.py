@@ -8,7 +8,9 @@ measured peak (the peaks file at the repository root, when present).
 
 Ops: fused_add_relu, gelu, silu, softmax, layer_norm, scan_rows, mamba_scan, transpose, slice,
 max_pool, conv1d_depthwise, dwconv_time_major, conv2d_tf32, conv2d_stem, conv2d_stem_pool, attention (--batch, --cols = sequence length, --m = model
-width), gemm.  Inputs are seeded random data; between timed
+width), gemm; serving attention (--batch sequences of --cols tokens, --m = model width in heads of 128, four
+to a kv head): attention_prompt, attention_decode (one new token each, --dtype f32 is taken as e4m3), attention_chunk
+(--rows new tokens each), kv_cache_write and kv_cache_read (e4m3).  Inputs are seeded random data; between timed
 launches nothing is flushed, so choose sizes larger than the 126 MB L2 for HBM figures.  This is
 also the command the ncu captures summarised under profiles/ were taken with.
 """
@@ -58,6 +60,57 @@ def _time(fn, iters, warm):
     ms = capi.c_float(0)
     capi.check(lib.fb200_event_elapsed_ms(e0, e1, capi.byref(ms)))
     return ms.value / iters
+
+
+def _serving(a, rng):
+    """The serving attention ops over equal sequences; pages of 64 tokens in random order."""
+    n, length, heads, d, page = a.batch, a.cols, a.m // 128, 128, 64
+    kv = max(1, heads // 4)
+    new = {"attention_decode": 1, "attention_chunk": a.rows}.get(a.op, length)
+    coded = a.op.startswith("kv_cache") or a.dtype != "bf16"
+    rows, tokens = n * new, n * length
+    offsets = lambda step: capi.DeviceBuffer.from_numpy((np.arange(n + 1) * step).astype(np.int32))
+    p = capi.AttentionParams(n_seqs=n, heads=heads, kv_heads=kv, head_dim=d, q_rows=rows, kv_rows=tokens, max_q=new,
+                             max_kv=length, q_token_stride=heads * d, q_head_stride=d, o_token_stride=heads * d,
+                             o_head_stride=d, k_token_stride=kv * d, k_head_stride=d, v_token_stride=kv * d,
+                             v_head_stride=d, scale=d ** -0.5, causal=1, dtype=capi.BF16)
+    flops = 4.0 * heads * d * n * (new * length - new * (new - 1) // 2)
+    if a.op == "attention_prompt":
+        q, k, v = (_rand((tokens, h, d), capi.BF16, rng) for h in (heads, kv, kv))
+        o, cu = capi.DeviceBuffer(tokens * heads * d * 2), offsets(length)
+        return (lambda: capi.attention_prompt(p, q.ptr, k.ptr, v.ptr, o.ptr, cu.ptr, cu.ptr)), \
+            2 * tokens * d * (2 * heads + 2 * kv), flops
+    per_seq = -(-length // page)
+    pages = n * per_seq
+    table = capi.DeviceBuffer.from_numpy(rng.permutation(pages).astype(np.int32))
+    size = pages * kv * page * d
+    both = [capi.DeviceBuffer.from_numpy(rng.integers(0, 126, size, dtype=np.uint8)) if coded else _rand((size,), capi.BF16, rng)
+            for _ in range(2)]
+    cache = capi.KvCache(k=both[0].ptr, v=both[1].ptr, pages=pages, page_size=page, kv_heads=kv, head_dim=d,
+                         page_stride=kv * page * d, token_stride=d, head_stride=page * d, dtype=capi.U8 if coded else capi.BF16)
+    if coded:
+        scales = [capi.DeviceBuffer.from_numpy(np.full(pages * kv * page, 118, dtype=np.uint8)) for _ in range(2)]
+        cache.k_scale, cache.v_scale = scales[0].ptr, scales[1].ptr
+        cache.scale_page_stride, cache.scale_token_stride, cache.scale_head_stride = kv * page, 1, page
+        both += scales
+    stored = 2 * tokens * kv * (d + 1 if coded else 2 * d)
+    lens = capi.DeviceBuffer.from_numpy(np.full(n, length, dtype=np.int32))
+    if a.op.startswith("kv_cache"):
+        k, v, cu = _rand((tokens, kv, d), capi.BF16, rng), _rand((tokens, kv, d), capi.BF16, rng), offsets(length)
+        keep = (both, k, v, cu, lens, table)
+        if a.op == "kv_cache_write":
+            fn = lambda: keep and capi.kv_cache_write(cache, k.ptr, kv * d, d, v.ptr, kv * d, d, cu.ptr, lens.ptr, table.ptr,
+                                                      per_seq, n, tokens, capi.BF16)
+        else:
+            fn = lambda: keep and capi.kv_cache_read(cache, k.ptr, kv * d, d, v.ptr, kv * d, d, cu.ptr, table.ptr, per_seq, n,
+                                                     tokens, capi.BF16)
+        return fn, stored + 2 * tokens * kv * 2 * d, 0.0
+    q, o, cu = _rand((rows, heads, d), capi.BF16, rng), capi.DeviceBuffer(rows * heads * d * 2), offsets(new)
+    need = capi.attention_paged_workspace(p, cache)
+    work = capi.DeviceBuffer.from_numpy(np.zeros(max(need, 1), dtype=np.uint8))
+    keep = (both, lens, table)
+    return (lambda: keep and capi.attention_paged(p, cache, q.ptr, o.ptr, cu.ptr, lens.ptr, table.ptr, per_seq, work.ptr, need)), \
+        stored + 4 * rows * heads * d, flops
 
 
 def main():
@@ -178,6 +231,8 @@ def main():
                                         tab.ptr, len(table), seq, seq, 64, capi.BF16)
         nbytes = 4 * bt * seq * width * 2
         flops = 4.0 * bt * heads * seq * seq * 64
+    elif a.op in ("attention_prompt", "attention_decode", "attention_chunk", "kv_cache_write", "kv_cache_read"):
+        fn, nbytes, flops = _serving(a, rng)
     elif a.op == "gemm":
         m, n, k = a.m, a.n, a.k
         x, w, o = _rand((m, k), dt, rng), _rand((k, n), dt, rng), capi.DeviceBuffer(m * n * es)

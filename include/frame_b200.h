@@ -418,8 +418,9 @@ FB200_API int fb200_attention_fan(const void* q_base, int64_t q_rows, int64_t q_
  * a row that sees no key is all zeros (its lse -infinity).  Products and softmax statistics are
  * fp32; probabilities are rounded to 16 bits before the second product (as in attention_fan), O once
  * at the store.  lse (optional, fp32 [q_rows, heads]): log of the row's sum of exp(scale * score).
- * A key that a row does not see does not reach it, whatever its K holds; in 16-bit V a NaN or an
- * infinity of a later key of the SAME sequence may reach earlier rows of its 128-key tile.
+ * A key that a row does not see does not reach it, whatever its K holds, and nothing behind a
+ * sequence's last key does; but a NaN or an infinity in V of a later key of the SAME sequence may
+ * reach earlier rows of its 128-key tile (their probability of zero times it).
  * Layouts: element strides per token and per head, head_dim contiguous; every base 16-byte aligned,
  * every stride a multiple of 8 elements (16 for e4m3 codes).  dtype BF16 or F16; head_dim a
  * multiple of 16 up to 128; heads a multiple of kv_heads, heads / kv_heads <= 64.  Anything else

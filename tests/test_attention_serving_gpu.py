@@ -316,3 +316,232 @@ def test_a_conversation_prompt_then_chunks_then_single_tokens(coded):
         tol, _ = ref.bounds(o, mag, arg, dt, d, coded)
         got = ref.load(np.concatenate(rows_of[s]), dt)
         assert np.all(np.abs(got - o) <= tol), float(np.max(np.abs(got - o) / tol))
+
+
+# ---- how the calls are made ---------------------------------------------------------------------------
+class Call:
+    """A paged call whose pieces stay on the device."""
+
+    def __init__(self, rng, dt, h, hk, d, lq, lk, page=16, coded=False, rows=None):
+        self.dt, self.h, self.d, self.lq, self.lk, self.coded = dt, h, d, lq, lk, coded
+        self.pages = ref.Pages(rng, lk, page, hk, d, dt, coded, True)
+        for s, n in enumerate(lk):
+            self.pages.put(s, 0, ref.store(rng.standard_normal((n, hk, d)), dt), ref.store(rng.standard_normal((n, hk, d)), dt))
+        self.cu, self.scale = ref.offsets(lq), 1.0 / np.sqrt(d)
+        self.rows = rows or int(self.cu[-1])
+        self.q = ref.store(rng.standard_normal((self.rows, h, d)), dt)
+        self.p = params(dt, h, hk, d, lq, lk, self.rows, 1, self.scale)
+        self.cache = self.pages.upload()
+        self.size = capi.attention_paged_workspace(self.p, self.cache)
+        self.work = upload(np.zeros(max(self.size, 1), dtype=np.uint8))
+        self.dq, self.dcu, self.dlen = upload(self.q), upload(self.cu), upload(np.array(lk, dtype=np.int32))
+        self.out, self.lse = upload(np.full(self.q.shape, FILL, dtype=np.uint16)), capi.DeviceBuffer(self.rows * h * 4)
+
+    def run(self, stream=None):
+        capi.attention_paged(self.p, self.cache, self.dq.ptr, self.out.ptr, self.dcu.ptr, self.dlen.ptr,
+                             self.pages.dev["table"].ptr, self.pages.table.shape[1], self.work.ptr, self.size,
+                             lse=self.lse.ptr, stream=stream)
+
+    def got(self):
+        return self.out.download(np.uint16, self.q.shape)
+
+    def check(self, lk=None):
+        seqs = [tuple(self.pages.values(s, n)) for s, n in enumerate(lk or self.lk)]
+        check_rows(self.got(), self.lse.download(np.float32, self.q.shape[:2]).astype(np.float64), self.q, self.cu, seqs, self.dt,
+                   self.d, np.float32(self.scale), 1, self.coded)
+
+
+@pytest.mark.parametrize("lq", [1, 30], ids=["decode", "chunk"])
+@pytest.mark.parametrize("coded", [False, True], ids=["same", "e4m3"])
+def test_many_sequences(lq, coded):
+    """More sequences than a warp has lanes, some without rows, some without keys."""
+    rng = np.random.default_rng(21)
+    lens = [int(n) for n in rng.integers(0, 260, 101)]
+    call = Call(rng, BF, 4, 2, 64, [0 if i % 7 == 3 else min(lq, 1 + i % lq) for i in range(101)], lens, coded=coded)
+    call.run()
+    capi.synchronize()
+    assert capi.kernel_status(0) == 0
+    call.check()
+
+
+def test_many_prompts():
+    dt, h, hk, d = FH, 4, 2, 64
+    rng = np.random.default_rng(22)
+    lens = [int(n) for n in rng.integers(0, 300, 77)]
+    cu = ref.offsets(lens)
+    rows = int(cu[-1])
+    q, k, v = (ref.store(rng.standard_normal((rows, n, d)), dt) for n in (h, hk, hk))
+    p = params(dt, h, hk, d, lens, lens, rows, 1, 0.125)
+    p.kv_rows, p.k_token_stride, p.k_head_stride, p.v_token_stride, p.v_head_stride = rows, hk * d, d, hk * d, d
+    dq, dk, dv, dcu, out = upload(q), upload(k), upload(v), upload(cu), upload(np.full(q.shape, FILL, dtype=np.uint16))
+    lse = capi.DeviceBuffer(rows * h * 4)
+    capi.attention_prompt(p, dq.ptr, dk.ptr, dv.ptr, out.ptr, dcu.ptr, dcu.ptr, lse=lse.ptr)
+    capi.synchronize()
+    assert capi.kernel_status(0) == 0
+    seqs = [(ref.load(k[cu[s]:cu[s + 1]], dt), ref.load(v[cu[s]:cu[s + 1]], dt)) for s in range(len(lens))]
+    check_rows(out.download(np.uint16, q.shape), lse.download(np.float32, (rows, h)).astype(np.float64), q, cu, seqs, dt, d,
+               np.float32(0.125), 1)
+
+
+def test_calls_on_two_streams_do_not_disturb_each_other():
+    rng = np.random.default_rng(23)
+    calls = [Call(rng, BF, 16, 2, 128, [1] * 5, [2000, 30, 900, 5, 1500]), Call(rng, BF, 16, 2, 128, [40, 3], [3000, 1100])]
+    streams = []
+    for _ in calls:
+        streams.append(capi.c_void_p())
+        capi.check(capi.load().fb200_stream_create(0, capi.byref(streams[-1])))
+    for _ in range(20):
+        for c, s in zip(calls, streams):
+            c.run(s)
+    for c, s in zip(calls, streams):
+        capi.synchronize(0, s)
+        c.check()
+        capi.check(capi.load().fb200_stream_destroy(0, s))
+    assert capi.kernel_status(0) == 0
+
+
+@pytest.mark.parametrize("lq", [[1, 1, 1], [40, 1, 17]], ids=["decode", "chunk"])
+def test_captured_and_replayed_with_lengths_that_grow_on_the_device(lq):
+    """The launches depend on max_q and max_kv only: a captured step is replayed while kv_len changes."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(24)
+    top = [1800, 700, 60]
+    call = Call(rng, BF, 8, 2, 128, lq, top)
+    call.run()
+    capi.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        call.run(torch.cuda.current_stream().cuda_stream)
+    for lens in ([40, 1, 17], [900, 300, 18], top):
+        call.dlen.upload(np.array(lens, dtype=np.int32))
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert capi.kernel_status(0) == 0
+        call.check(lens)
+
+
+def test_more_rows_than_max_q_are_recorded_and_offsets_are_cut():
+    rng = np.random.default_rng(25)
+    for lq, most in ([3, 2], 1), ([40, 2], 20):            # the bound of either kernel
+        call = Call(rng, BF, 4, 2, 64, lq, [50, 20])
+        call.p.max_q = most
+        call.run()
+        capi.synchronize()
+        assert capi.kernel_status(0) == 322
+    call = Call(rng, BF, 4, 2, 64, [3, 2], [50, 20])
+    for cu in ([0, 3, 1 << 30], [-7, 3, 5], [4, 2, 5]):    # past the rows, negative, falling
+        call.dcu.upload(np.array(cu, dtype=np.int32))
+        call.dlen.upload(np.array([1 << 30, -4], dtype=np.int32))
+        call.run()
+        capi.synchronize()
+        capi.kernel_status(0)
+    call = Call(rng, BF, 4, 2, 64, [3, 2], [50, 20])       # and the device is as it was
+    call.run()
+    capi.synchronize()
+    assert capi.kernel_status(0) == 0
+    call.check()
+
+
+@pytest.mark.parametrize("dt", [BF, FH])
+@pytest.mark.parametrize("lq", [1, 20], ids=["decode", "chunk"])
+def test_what_a_row_does_not_see_does_not_reach_it(dt, lq):
+    """NaN and infinity in K of later tokens, and in K and V of tokens behind the sequence's length."""
+    rng = np.random.default_rng(26)
+    n, h, hk, d = 300, 8, 2, 64
+    call = Call(rng, dt, h, hk, d, [lq], [n])
+    clean = [x.copy() for x in call.pages.values(0, n)]
+    at = call.pages.put
+    k, v = (ref.store(x, dt) for x in clean)
+    bad = k.copy()
+    bad[n - 1] = NAN[dt]                                   # the last query alone sees it
+    at(0, 0, bad, v)
+    call.pages.dev["k"].upload(call.pages.k)
+    call.run()
+    capi.synchronize()
+    got = ref.load(call.got(), dt)
+    assert np.all(np.isnan(got[lq - 1]))
+    o, _, mag, arg = ref.attention(ref.load(call.q, dt), clean[0], clean[1], np.float32(call.scale), True)
+    tol, _ = ref.bounds(o, mag, arg, dt, d)
+    assert np.all(np.abs(got[:lq - 1] - o[:lq - 1]) <= tol[:lq - 1])
+    bad_v = v.copy()
+    bad_v[n - 5:] = NAN[dt]                                # behind the length from now on
+    at(0, 0, bad, bad_v)
+    for name in "kv":
+        call.pages.dev[name].upload(getattr(call.pages, name))
+    call.dlen.upload(np.array([n - 5], dtype=np.int32))
+    call.run()
+    capi.synchronize()
+    o, _, mag, arg = ref.attention(ref.load(call.q, dt), clean[0][:n - 5], clean[1][:n - 5], np.float32(call.scale), True)
+    tol, _ = ref.bounds(o, mag, arg, dt, d)
+    assert np.all(np.abs(ref.load(call.got(), dt) - o) <= tol)
+    assert capi.kernel_status(0) == 0
+
+
+def test_an_e4m3_token_stored_as_not_finite_makes_the_rows_that_see_it_nan():
+    rng = np.random.default_rng(27)
+    for lq in (1, 20):
+        call = Call(rng, BF, 8, 2, 64, [lq, lq], [300, 200], coded=True)
+        ids, tok = call.pages.table[0, 7 // 16], 7
+        call.pages.vs[ids, :, tok] = 255                   # value of token 7 of the first sequence
+        call.pages.dev["vs"].upload(call.pages.vs)
+        call.run()
+        capi.synchronize()
+        got = ref.load(call.got(), BF)
+        assert np.all(np.isnan(got[:lq])) and not np.any(np.isnan(got[lq:]))
+
+
+@pytest.mark.parametrize("lq", [1, 20], ids=["decode", "chunk"])
+@pytest.mark.parametrize("dt", [BF, FH])
+def test_value_scales_far_apart_keep_their_precision(dt, lq):
+    """e4m3 values whose scales span 2^20: each row is as near as its own weights allow."""
+    rng = np.random.default_rng(28)
+    n, h, hk, d = 400, 8, 2, 128
+    call = Call(rng, dt, h, hk, d, [lq], [n], coded=True)
+    gain = np.exp2(rng.integers(-14, 6, (n, hk, 1)))
+    v = ref.store(rng.standard_normal((n, hk, d)) * gain, dt)
+    v[5] = 0                                               # a row of zeros: scale 2^-126
+    call.pages.put(0, 0, ref.store(rng.standard_normal((n, hk, d)), dt), v)
+    for name in ("k", "v", "ks", "vs"):
+        call.pages.dev[name].upload(getattr(call.pages, name))
+    call.run()
+    capi.synchronize()
+    assert capi.kernel_status(0) == 0
+    call.check()
+
+
+@pytest.mark.parametrize("lq", [1, 40], ids=["decode", "chunk"])
+@pytest.mark.parametrize("coded", [False, True], ids=["same", "e4m3"])
+def test_pages_whose_offsets_pass_32_bits(lq, coded):
+    """Pages 2^28 bytes apart, the last at 5 GiB; keys and values in the same memory."""
+    dt, h, hk, d, page, n = BF, 8, 2, 128, 64, 200
+    rng = np.random.default_rng(29)
+    near = ref.Pages(rng, [n], page, hk, d, dt, coded, True, spare=0)
+    x = ref.store(rng.standard_normal((n, hk, d)), dt)
+    near.put(0, 0, x, x)
+    item = 1 if coded else 2
+    far = capi.DeviceBuffer((20 << 28) + (1 << 20))
+    spots = np.array([20, 3, 17, 9], dtype=np.int32)       # where the sequence's four pages go
+    for i, at in enumerate(spots):
+        one = np.ascontiguousarray(near.k[near.table[0, i]])
+        capi.check(capi.load().fb200_memcpy(0, far.ptr.value + (int(at) << 28), one.ctypes.data, one.nbytes, capi.H2D, None, 1))
+    cache = near.upload()
+    cache.k = cache.v = far.ptr
+    cache.pages, cache.page_stride = 21, (1 << 28) // item
+    if coded:                                              # the scales' pages move with them
+        scales = np.full((21, hk, page), 255, dtype=np.uint8)
+        scales[spots] = near.ks[near.table[0, :4]]
+        dscale = upload(scales)
+        cache.k_scale = cache.v_scale = dscale.ptr
+    table = upload(spots[None])
+    q = ref.store(rng.standard_normal((lq, h, d)), dt)
+    p = params(dt, h, hk, d, [lq], [n], lq, 1, 0.09)
+    size = capi.attention_paged_workspace(p, cache)
+    work, dq, out = upload(np.zeros(max(size, 1), dtype=np.uint8)), upload(q), upload(np.zeros(q.shape, dtype=np.uint16))
+    cu, dlen, lse = upload(np.array([0, lq], dtype=np.int32)), upload(np.array([n], dtype=np.int32)), capi.DeviceBuffer(lq * h * 4)
+    capi.attention_paged(p, cache, dq.ptr, out.ptr, cu.ptr, dlen.ptr, table.ptr, 4, work.ptr, size, lse=lse.ptr)
+    capi.synchronize()
+    assert capi.kernel_status(0) == 0
+    k, v = near.values(0, n)
+    check_rows(out.download(np.uint16, q.shape), lse.download(np.float32, (lq, h)).astype(np.float64), q, [0, lq], [(k, v)], dt, d,
+               np.float32(0.09), 1, coded)
