@@ -485,8 +485,8 @@ FB200_API int fb200_kv_cache_read(const fb200_kv_cache* cache, void* k, int64_t 
  * parts meet in `workspace` (fb200_attention_paged_workspace bytes, 256-byte aligned), which must be
  * zero before its first use, may be used by any later call on the same stream (every call leaves
  * the part that has to be zero so), and must not be shared by calls that overlap.  The parts are
- * joined in a fixed order: results do not depend on timing.  A key on a page number outside the cache
- * is taken from page 0 and recorded as kernel status 321. */
+ * joined in a fixed order: results do not depend on timing.  o must not overlap q.  A key on a page
+ * number outside the cache is taken from page 0 and recorded as kernel status 321. */
 FB200_API int fb200_attention_paged_workspace(const fb200_attention_params* params,
                                               const fb200_kv_cache* cache, size_t* bytes);
 FB200_API int fb200_attention_paged(const fb200_attention_params* params, const fb200_kv_cache* cache,
