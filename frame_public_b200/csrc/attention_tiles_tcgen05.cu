@@ -117,55 +117,61 @@ __device__ __forceinline__ int keys_seen(int causal, int end, int lq, int lk) {
 // that cost more than c tiles is a closed form per sequence; a binary search over c finds the cost of
 // the rank, a scan over the sequences the block.  Run by one warp; returns false past the last item.
 template <bool PAGED>
-__device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int rank, int tokens, TilesItem& item,
-                          int* status) {
+__device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int rank, int tokens, uint32_t tokens_inverse,
+                          TilesItem& item, int* status) {
   const int lane = threadIdx.x & 31;
-  // blocks of sequence (lq, lk) that see more than 128 * c keys
-  auto above = [&](int lq, int lk, int c) {
-    const int blocks = (lq + tokens - 1) / tokens;
-    if (c < 0) return blocks;
-    if (lk <= c * kTileKeys) return 0;
-    if (!p.causal) return blocks;
-    const int y = c * kTileKeys - lk + lq;   // blocks that end at or before token y see no more
-    return blocks - max(0, min(y >= 0 ? y / tokens : 0, blocks - 1));
+  // y / tokens for 0 <= y < 2^31: tokens_inverse = floor(2^32 / tokens) gives it or one less
+  auto over_tokens = [&](int y) {
+    const int q = static_cast<int>(__umulhi(static_cast<uint32_t>(y), tokens_inverse));
+    return q + (y - q * tokens >= tokens ? 1 : 0);
   };
-  int q0_mine = 0, lq_mine = 0, k0_mine = 0, lk_mine = 0;   // sequence `lane` stays in registers
-  if (lane < p.n_seqs) serving_lengths<PAGED>(p, cache, lane, q0_mine, lq_mine, k0_mine, lk_mine);
-  auto lengths = [&](int s, int& q0, int& lq, int& k0, int& lk) {
-    q0 = q0_mine, lq = lq_mine, k0 = k0_mine, lk = lk_mine;
-    if (s >= 32) serving_lengths<PAGED>(p, cache, s, q0, lq, k0, lk);
+  struct Seq {
+    int q0, lq, k0, lk, blocks;
   };
-  auto total = [&](int c, int& longest) {
-    int sum = 0, most = 0;
-    for (int s = lane; s < p.n_seqs; s += 32) {
-      int q0, lq, k0, lk;
-      lengths(s, q0, lq, k0, lk);
-      sum += above(lq, lk, c);
-      most = max(most, lk);
-      if (rank == 0 && c < 0 && lq > p.max_q) record_fault(status, kFaultBadLength);
+  auto load = [&](int s) {
+    Seq q{0, 0, 0, 0, 0};
+    if (s < p.n_seqs) {
+      serving_lengths<PAGED>(p, cache, s, q.q0, q.lq, q.k0, q.lk);
+      q.blocks = over_tokens(q.lq + tokens - 1);
     }
-    longest = __reduce_max_sync(0xffffffffu, most);
+    return q;
+  };
+  const Seq mine = load(lane);   // sequence `lane` stays in registers
+  auto sequence = [&](int s) { return s < 32 ? mine : load(s); };
+  // blocks of a sequence that see more than 128 * c keys
+  auto above = [&](const Seq& q, int c) {
+    if (c < 0) return q.blocks;
+    if (q.lk <= c * kTileKeys) return 0;
+    if (!p.causal) return q.blocks;
+    const int y = c * kTileKeys - q.lk + q.lq;   // blocks that end at or before token y see no more
+    return q.blocks - min(over_tokens(max(y, 0)), max(q.blocks - 1, 0));
+  };
+  auto total = [&](int c) {
+    int sum = above(mine, c);
+    for (int s = lane + 32; s < p.n_seqs; s += 32) sum += above(load(s), c);
     return __reduce_add_sync(0xffffffffu, sum);
   };
-  int longest = 0;
-  if (rank >= total(-1, longest)) return false;
+  int most = mine.lk, widest = mine.lq;
+  for (int s = lane + 32; s < p.n_seqs; s += 32) {
+    const Seq q = load(s);
+    most = max(most, q.lk);
+    widest = max(widest, q.lq);
+  }
+  if (rank == 0 && widest > p.max_q) record_fault(status, kFaultBadLength);
+  const int longest = __reduce_max_sync(0xffffffffu, most);
+  if (rank >= total(-1)) return false;
   int lo = -1, hi = (longest + kTileKeys - 1) / kTileKeys;   // total(lo) > rank >= total(hi)
-  int below = 0, ignored;                                    // total(hi)
+  int below = 0;                                             // total(hi)
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1, n = total(mid, ignored);
+    const int mid = (lo + hi) >> 1, n = total(mid);
     if (n > rank) lo = mid;
     else { hi = mid; below = n; }
   }
   // items of cost hi exactly, in sequence order: `rank - below` of them lie before this one
   int left = rank - below;
   for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
-    const int s = s0 + lane;
-    int q0 = 0, lq = 0, k0 = 0, lk = 0, n = 0, more = 0;
-    if (s < p.n_seqs) {
-      lengths(s, q0, lq, k0, lk);
-      more = above(lq, lk, hi);
-      n = above(lq, lk, hi - 1) - more;
-    }
+    const Seq q = sequence(s0 + lane);
+    const int more = above(q, hi), n = above(q, hi - 1) - more;
     int upto = n;   // inclusive scan
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -175,14 +181,13 @@ __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int 
     const uint32_t hit = __ballot_sync(0xffffffffu, upto > left);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      const int blocks = (lq + tokens - 1) / tokens;
-      const int block = blocks - more - n + (left - (upto - n));
+      const int block = q.blocks - more - n + (left - (upto - n));
       item.seq = s0 + src;
       item.block = __shfl_sync(0xffffffffu, block, src);
-      item.q0 = __shfl_sync(0xffffffffu, q0, src);
-      item.lq = __shfl_sync(0xffffffffu, lq, src);
-      item.k0 = __shfl_sync(0xffffffffu, k0, src);
-      item.lk = __shfl_sync(0xffffffffu, lk, src);
+      item.q0 = __shfl_sync(0xffffffffu, q.q0, src);
+      item.lq = __shfl_sync(0xffffffffu, q.lq, src);
+      item.k0 = __shfl_sync(0xffffffffu, q.k0, src);
+      item.lk = __shfl_sync(0xffffffffu, q.lk, src);
       return true;
     }
     left -= __shfl_sync(0xffffffffu, upto, 31);
@@ -220,7 +225,7 @@ template <typename T, int SPANS, bool PAGED, bool E4M3>
 __global__ void __launch_bounds__(tiles_threads(E4M3), 1)
 attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                        const __grid_constant__ CUtensorMap tmap_v, const ServingProblem p, const PagedCache cache,
-                       const TilesSplit split, int tile_tokens, int box_keys, int* status) {
+                       const TilesSplit split, int tile_tokens, uint32_t tokens_inverse, int box_keys, int* status) {
   using M = typename std::conditional<E4M3, __half, T>::type;   // type of the operands
   constexpr bool kLift = E4M3 && !std::is_same<T, __half>::value;   // the query rows become float16
   constexpr uint32_t kFmt = std::is_same<M, __half>::value ? kFmtF16 : kFmtBF16;
@@ -244,9 +249,11 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = blockIdx.x % split.parts, pair = blockIdx.x / split.parts, head = pair % p.kv_heads;
+  // of the softmax threads, worked out while the item is looked for
+  const int row = threadIdx.x & 127, in_tile = row / p.group;
   if (warp == 0) {
     TilesItem it;
-    const bool found = find_item<PAGED>(p, cache, pair / p.kv_heads, 2 * tile_tokens, it, status);
+    const bool found = find_item<PAGED>(p, cache, pair / p.kv_heads, 2 * tile_tokens, tokens_inverse, it, status);
     if (lane == 0) {
       if (found) *item_ptr = it;
       *found_ptr = found;
@@ -277,13 +284,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   tcgen05_fence_before_sync();
   __syncthreads();
   tcgen05_fence_after_sync();
-  // Equal in all lanes; a warp reduction leaves its result in a uniform register, which is where the
-  // descriptors, addresses and loop bounds of the tensor instructions have to be.
-  auto uniform = [](int x) { return __reduce_max_sync(0xffffffffu, x); };
   const uint32_t tmem = __reduce_max_sync(0xffffffffu, *tmem_slot_ptr);
-  const TilesItem item{uniform(item_ptr->seq), uniform(item_ptr->block), uniform(item_ptr->q0),
-                       uniform(item_ptr->lq), uniform(item_ptr->k0), uniform(item_ptr->lk)};
-  const bool found = uniform(*found_ptr) != 0;
+  const TilesItem item = *item_ptr;
+  const bool found = *found_ptr != 0;
   const int token0 = item.block * 2 * tile_tokens;
   int tiles[2];   // of keys that each stage's rows see
 #pragma unroll
@@ -440,7 +443,11 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     // Straight-line issue: descriptors and ring positions advance by additions in warp-uniform code (a
     // division per tile and a rolled loop over the k steps took 2900 cycles per 128 x 128 x 128 pair of
     // products, three times what the tensor core needs for it).
-    if (most > 0) {
+    // Equal in all lanes; a warp reduction leaves its result in a uniform register, which is where the
+    // descriptors, addresses and loop bounds of the tensor instructions have to be.
+    auto uniform = [](int x) { return __reduce_max_sync(0xffffffffu, x); };
+    const int u_most = uniform(most), u_tiles[2] = {uniform(tiles[0]), uniform(tiles[1])}, keys_left = uniform(item.lk - key0);
+    if (u_most > 0) {
       const int k_steps = p.dim / 16;
       const uint32_t idesc_s = make_instr_desc(kFmt, 0, 0, kTileRows, kTileKeys);
       const uint32_t idesc_o = make_instr_desc(kFmt, 0, 1, kTileRows, static_cast<uint32_t>(p.dim));
@@ -482,18 +489,18 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       live = live && mbar_wait_lanes(full, 0, status, kFaultTilesKeys);
       tcgen05_fence_after_sync();
       if (live) {
-        if (tiles[0] > 0) scores(0);
-        if (tiles[1] > 0) scores(1);
+        if (u_tiles[0] > 0) scores(0);
+        if (u_tiles[1] > 0) scores(1);
         mma_commit_elect(freed);
         kp.next(kSlots);
       }
-      for (int j = 0; live && j < most; ++j) {
-        const bool more = j + 1 < most;
+      for (int j = 0; live && j < u_most; ++j) {
+        const bool more = j + 1 < u_most;
         if (kApart && more) live = mbar_wait_lanes(full + 8 * kp.slot, kp.phase, status, kFaultTilesKeys);
         if (kApart && more && live) {
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            if (j + 1 >= tiles[s]) continue;
+            if (j + 1 >= u_tiles[s]) continue;
             live = live && mbar_wait_lanes(bar_r + 8 * s, j & 1, status, kFaultTilesScores);
             tcgen05_fence_after_sync();
             if (live) scores(s);
@@ -501,7 +508,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         }
         live = live && mbar_wait_lanes(full + 8 * vp.slot, vp.phase, status, kFaultTilesKeys);
         if (!live) break;
-        const int there = item.lk - key0 - j * kTileKeys;
+        const int there = keys_left - j * kTileKeys;
         if (!E4M3 && there < kTileKeys) {
           // Rows behind the last key hold another sequence's values or none: their P is 0, but 0 times a
           // NaN is not.
@@ -515,9 +522,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          if (live && j < tiles[s]) values(s, j);
+          if (live && j < u_tiles[s]) values(s, j);
           if (!kApart && s == 0 && more) live = live && mbar_wait_lanes(full + 8 * kp.slot, kp.phase, status, kFaultTilesKeys);
-          if (!kApart && live && j + 1 < tiles[s]) scores(s);
+          if (!kApart && live && j + 1 < u_tiles[s]) scores(s);
         }
         if (!live) break;
         mma_commit_elect(freed + 8 * vp.slot);
@@ -531,8 +538,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     __syncwarp();
   } else {
     // ---- softmax ---------------------------------------------------------------------------------
-    const int s = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & 127;
-    const int in_tile = row / p.group, token = token0 + s * tile_tokens + in_tile;
+    const int s = warp >> 3, half = (warp >> 2) & 1, token = token0 + s * tile_tokens + in_tile;
     const int h = head * p.group + row - in_tile * p.group;
     const bool there = work && in_tile < tile_tokens && token < item.lq;
     const int limit = there ? keys_seen(p.causal, token + 1, item.lq, item.lk) - key0 : 0;   // keys this row sees from key0 on
@@ -706,26 +712,45 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       tcgen05_fence_after_sync();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const int64_t at = static_cast<int64_t>(item.q0 + token) * p.heads + h;
-      T* const dst = reinterpret_cast<T*>(p.o) + static_cast<int64_t>(item.q0 + token) * p.o_token + h * p.o_head;
+      // Rows go out through the stage's Q tile, which nothing reads any more (the last product is done, and the
+      // scores before it): a warp that stored its 32 rows from registers, 16 bytes of each at a time, took
+      // 3 K cycles a tile at head_dim 128.
+      uint8_t* const rows = base_ptr + s * kSlotBytes;
       for (int i = half * 16; i < p.dim; i += 32) {
         uint32_t x[16];
         if (any) {
           tmem_ld_32x32b_x16(t_o + i, x);
           tmem_ld_wait(x);
         }
-        if (!there) continue;
         if (parted) {
           float* const to = split.o + (part * static_cast<int64_t>(p.q_rows) * p.heads + at) * p.dim + i;
 #pragma unroll
-          for (int e = 0; any && e < 16; e += 4) *reinterpret_cast<uint4*>(to + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+          for (int e = 0; there && any && e < 16; e += 4) *reinterpret_cast<uint4*>(to + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
         } else {
           uint32_t out[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             out[e] = l == 0.0f ? 0u : pack_pair<T>(__uint_as_float(x[2 * e]) * inv, __uint_as_float(x[2 * e + 1]) * inv);
           }
-          *reinterpret_cast<uint4*>(dst + i) = make_uint4(out[0], out[1], out[2], out[3]);
-          *reinterpret_cast<uint4*>(dst + i + 8) = make_uint4(out[4], out[5], out[6], out[7]);
+          uint8_t* const to = rows + (i >> 6) * kSpanBytes + row * 128;
+          const int chunk = (i >> 3) & 7;
+          *reinterpret_cast<uint4*>(to + ((chunk ^ (row & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+          *reinterpret_cast<uint4*>(to + (((chunk + 1) ^ (row & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
+        }
+      }
+      if (!parted) {
+        live = pair_sync(live);   // both halves of the 32 rows are there; each warp stores 16 of them
+        const int64_t to = (static_cast<int64_t>(item.q0 + token) * p.o_token + h * p.o_head) * 2;
+        constexpr int kChunks = SPANS * 8, kRowsAtOnce = 32 / kChunks;
+        const int chunk = lane % kChunks;
+#pragma unroll
+        for (int i = 0; i < 16 / kRowsAtOnce; ++i) {
+          const int from = half * 16 + i * kRowsAtOnce + lane / kChunks;   // lane that knows the row
+          const int r = (warp & 3) * 32 + from;
+          const int64_t dst = __shfl_sync(0xffffffffu, to, from);
+          const bool wanted = __shfl_sync(0xffffffffu, there ? 1 : 0, from) != 0;
+          const uint4 x = *reinterpret_cast<const uint4*>(rows + (chunk >> 3) * kSpanBytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
+          if (wanted && chunk * 8 < p.dim) *reinterpret_cast<uint4*>(p.o + dst + chunk * 16) = x;
         }
       }
       if (there && half == 0) {
@@ -860,7 +885,8 @@ int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, boo
     const size_t smem = ((tiles_small_bytes(spans, e4m3) + 1023) & ~1023u) + static_cast<size_t>(spans * kSpanBytes) * (2 + tiles_slots(spans, e4m3)) + (e4m3 ? kRawSlots * kSpanBytes : 0);
     static SmemOptIn opted;
     if (int rc = opted.once(kernel, smem)) return rc;
-    kernel<<<static_cast<unsigned>(grid), tiles_threads(e4m3), smem, stream>>>(tq, tk, tv, p, view, split, tile_tokens, box_keys, status);
+    kernel<<<static_cast<unsigned>(grid), tiles_threads(e4m3), smem, stream>>>(tq, tk, tv, p, view, split, tile_tokens,
+                                                                             static_cast<uint32_t>((uint64_t(1) << 32) / (2 * tile_tokens)), box_keys, status);
     return FB200_OK;
   };
   auto pick = [&](auto type) -> int {
