@@ -72,9 +72,9 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // 2^x without the XU pipe: x = n + f with f in [-1/2, 1/2] by adding 1.5 * 2^23 (n stands in the low bits of
 // the sum), 2^f by the polynomial of degree 5 with the least largest relative error (1.6e-7 in fp32
-// arithmetic; found by reweighted least squares, constant term 1), n added to its exponent.  From -127 down:
-// f = 0 and the exponent field becomes 0, which is exactly 0.  A NaN stays in the maximum and ends as the
-// largest number, which becomes an infinity in P and NaN in O.
+// arithmetic; found by reweighted least squares, constant term 1), times 2^n from its exponent field.  From
+// -127 down that field is 0, and so is the result.  A NaN stays one in every step: whatever the bits of n are
+// then, the last one multiplies with them (adding n to the polynomial's exponent made a finite number of it).
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
   asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));   // -127
   asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
@@ -88,9 +88,8 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
     y = fmaf(y, z, 0.693147f);
     return fmaf(y, z, 1.0f);
   };
-  const float2 y = make_float2(poly(f.x), poly(f.y));
-  return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
+  auto power = [](float z) { return __uint_as_float((__float_as_uint(z) << 23) + 0x3F800000u); };
+  return __fmul2_rn(make_float2(poly(f.x), poly(f.y)), make_float2(power(t.x), power(t.y)));
 }
 template <typename T> __device__ __forceinline__ uint32_t pack_pair(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float lo, float hi) {

@@ -1,0 +1,109 @@
+"""Attention of packed prompts and over a paged cache where numbers and lengths are at their edges: NaN at
+every place of a tile, parts that hold nothing else, the top and the bottom of the types, more rows than
+max_q, lengths that leave the extents, calls large enough for the wide forms of the cache's write and read."""
+import numpy as np
+import pytest
+
+import serving_ref as ref
+from frame_public_b200 import capi
+from test_attention_serving_gpu import BF, FH, FILL, NAN, Call, check_rows, params, upload
+
+pytestmark = pytest.mark.gpu
+
+
+class Prompt:
+    """A prompt call whose pieces stay on the device; k and v default to random numbers."""
+
+    def __init__(self, rng, dt, h, hk, d, lq, lk=None, scale=None, causal=1, q=None, k=None, v=None):
+        lk = lk or lq
+        self.dt, self.d, self.lq, self.lk, self.causal = dt, d, lq, lk, causal
+        self.cu, self.cuk = ref.offsets(lq), ref.offsets(lk)
+        rows, krows = int(self.cu[-1]), int(self.cuk[-1])
+        self.q = ref.store(rng.standard_normal((rows, h, d)), dt) if q is None else q
+        self.k = ref.store(rng.standard_normal((krows, hk, d)), dt) if k is None else k
+        self.v = ref.store(rng.standard_normal((krows, hk, d)), dt) if v is None else v
+        self.scale = scale or 1.0 / np.sqrt(d)
+        self.p = params(dt, h, hk, d, lq, lk, rows, causal, self.scale)
+        self.p.kv_rows = krows
+        self.p.k_token_stride, self.p.k_head_stride, self.p.v_token_stride, self.p.v_head_stride = hk * d, d, hk * d, d
+        self.dcu, self.dcuk = upload(self.cu), upload(self.cuk)
+
+    def run(self):
+        dq, dk, dv = upload(self.q), upload(self.k), upload(self.v)
+        out, lse = upload(np.full(self.q.shape, FILL, dtype=np.uint16)), capi.DeviceBuffer(self.q.shape[0] * self.q.shape[1] * 4)
+        capi.attention_prompt(self.p, dq.ptr, dk.ptr, dv.ptr, out.ptr, self.dcu.ptr, self.dcuk.ptr, lse=lse.ptr)
+        capi.synchronize()
+        return out.download(np.uint16, self.q.shape), lse.download(np.float32, self.q.shape[:2]).astype(np.float64)
+
+
+def resend(call):
+    """The call's cache as it stands on the host, and its query rows."""
+    for name in ("k", "v") + (("ks", "vs") if call.coded else ()):
+        call.pages.dev[name].upload(getattr(call.pages, name))
+    call.dq.upload(call.q)
+
+
+def run(call, status=0):
+    call.run()
+    capi.synchronize()
+    assert capi.kernel_status(0) == status
+    return ref.load(call.got(), call.dt), call.lse.download(np.float32, call.q.shape[:2]).astype(np.float64)
+
+
+def near(got, lse, q, k, v, dt, d, scale, coded=False, causal=True):
+    """Rows of one sequence against 64 bits."""
+    o, l, mag, arg = ref.attention(ref.load(q, dt), k, v, np.float32(scale), causal)
+    tol, tol_l = ref.bounds(o, mag, arg, dt, d, coded)
+    assert np.all(np.abs(got - o) <= tol), float(np.max(np.abs(got - o) / tol))
+    assert np.all(np.abs(lse - l) <= tol_l + 2.0 ** -22 * np.abs(l))
+
+
+def poison_key(call, seq, key, value_too=False):
+    """Token `key` of a sequence as one whose K is not finite; its V stays finite, zero on demand."""
+    at = call.pages._at(call.pages.k, seq, np.array([key]))
+    if call.coded:
+        call.pages.ks[at] = 255
+        call.pages.k[at] = 0
+    else:
+        call.pages.k[at] = NAN[call.dt]
+    if value_too:
+        call.pages.v[at] = 0
+        if call.coded:
+            call.pages.vs[at] = 1
+
+
+# ---- NaN ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("lq", [1, 3, 20], ids=["decode", "draft", "chunk"])
+@pytest.mark.parametrize("dt,d,coded", [(BF, 64, False), (FH, 128, False), (BF, 128, True), (FH, 64, True)])
+def test_a_key_that_is_not_finite_makes_the_rows_that_see_it_nan_at_every_place(dt, d, coded, lq):
+    """Places 32 .. 47 of a tile in turn, one sequence each; half of the values are zero."""
+    rng = np.random.default_rng(31)
+    call = Call(rng, dt, 8, 2, d, [lq] * 17, [200] * 17, coded=coded)
+    for r in range(16):
+        poison_key(call, r, 32 + r, r % 2 == 1)
+    resend(call)
+    got, lse = run(call)
+    for r in range(16):
+        rows = slice(r * lq, (r + 1) * lq)
+        assert np.all(np.isnan(got[rows])) and np.all(np.isnan(lse[rows])), r
+    rows = slice(16 * lq, 17 * lq)                         # and the last sequence does not know of it
+    near(got[rows], lse[rows], call.q[rows], *call.pages.values(16, 200), dt, d, call.scale, coded)
+
+
+@pytest.mark.parametrize("dt,d", [(BF, 64), (FH, 64), (BF, 128), (FH, 96)])
+def test_a_nan_key_of_a_prompt_reaches_the_rows_from_its_own_on(dt, d):
+    rng = np.random.default_rng(32)
+    n = 150
+    call = Prompt(rng, dt, 4, 2, d, [n] * 16)
+    for r in range(16):
+        call.k[r * n + 33 + r] = NAN[dt]
+    got, lse = call.run()
+    assert capi.kernel_status(0) == 0
+    got = ref.load(got, dt)
+    for r in range(16):
+        rows, at = slice(r * n, (r + 1) * n), 33 + r
+        assert np.all(np.isnan(got[rows][at:])) and np.all(np.isnan(lse[rows][at:])), r
+        near(got[rows][:at], lse[rows][:at], call.q[rows][:at], ref.load(call.k[rows][:at], dt), ref.load(call.v[rows][:at], dt),
+             dt, d, call.scale)
+
+
