@@ -793,7 +793,9 @@ __global__ void __launch_bounds__(256) attention_tiles_join_kernel(const Serving
 #pragma unroll 4
   for (int i = 0; i < parts; ++i) {
     const float2 ml = split.stats[i * stride + at];
-    if (ml.x == -INFINITY) continue;   // saw no key: nothing was stored
+    // Saw no key.  (A part whose scores are all NaN has no maximum either, but its sum is NaN and reaches the
+    // result: ex2(-inf - m) is 0 or NaN.)
+    if (ml.x == -INFINITY && ml.y == 0.0f) continue;
     const float f = ex2(ml.x - m);
     l += f * ml.y;
     if (mine) {

@@ -107,3 +107,28 @@ def test_a_nan_key_of_a_prompt_reaches_the_rows_from_its_own_on(dt, d):
              dt, d, call.scale)
 
 
+@pytest.mark.parametrize("dt,coded", [(BF, False), (FH, False), (BF, True), (FH, True)])
+def test_parts_that_hold_nothing_but_nan_are_not_taken_for_empty(dt, coded):
+    """A chunk whose keys are cut into parts: a NaN query row, and NaN in every key of some part."""
+    rng = np.random.default_rng(33)
+    h, hk, d, n, lq = 8, 2, 128, 6000, 20
+    call = Call(rng, dt, h, hk, d, [lq], [n], page=64, coded=coded)
+    assert call.size > 4096                                # the parts' room: this call is cut
+    clean = call.q.copy()
+    call.q[5, 3] = NAN[dt]
+    resend(call)
+    got, lse = run(call)
+    nan = np.zeros((lq, h), dtype=bool)
+    nan[5, 3] = True
+    assert np.array_equal(np.isnan(lse), nan) and np.array_equal(np.isnan(got), np.broadcast_to(nan[..., None], got.shape))
+    o, l, mag, arg = ref.attention(ref.load(clean, dt), *call.pages.values(0, n), np.float32(call.scale), True)
+    tol, tol_l = ref.bounds(o, mag, arg, dt, d, coded)
+    assert np.all((np.abs(got - o) <= tol)[~nan]) and np.all((np.abs(lse - l) <= tol_l + 2.0 ** -22 * np.abs(l))[~nan])
+    call.q = clean
+    for key in range(2048, 4096):                          # whole parts of 1024 and 2048 keys
+        poison_key(call, 0, key)
+    resend(call)
+    got, lse = run(call)
+    assert np.all(np.isnan(got)) and np.all(np.isnan(lse))
+
+
