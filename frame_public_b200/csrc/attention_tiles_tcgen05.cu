@@ -103,7 +103,7 @@ template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float lo, floa
 
 // A CTA's share of the work.
 struct TilesItem {
-  int seq, block, q0, lq, k0, lk;
+  int seq, block, q0, lq, rows, k0, lk;   // rows: of the lq query rows, those that are computed
 };
 
 // Keys that the block ending before token `end` sees.
@@ -114,7 +114,8 @@ __device__ __forceinline__ int keys_seen(int causal, int end, int lq, int lk) {
 // Item `rank` of the blocks of `tokens` query tokens of all sequences in order of falling cost (tiles of
 // keys): the long ones start first, so that the last CTAs to run are short ones.  The number of blocks
 // that cost more than c tiles is a closed form per sequence; a binary search over c finds the cost of
-// the rank, a scan over the sequences the block.  Run by one warp; returns false past the last item.
+// the rank, a scan over the sequences the block.  A sequence has blocks for its first max_q rows only, so that
+// one with more rows takes no other's place in the grid.  Run by one warp; returns false past the last item.
 template <bool PAGED>
 __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int rank, int tokens, uint32_t tokens_inverse,
                           TilesItem& item, int* status) {
@@ -125,13 +126,14 @@ __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int 
     return q + (y - q * tokens >= tokens ? 1 : 0);
   };
   struct Seq {
-    int q0, lq, k0, lk, blocks;
+    int q0, lq, rows, k0, lk, blocks;
   };
   auto load = [&](int s) {
-    Seq q{0, 0, 0, 0, 0};
+    Seq q{0, 0, 0, 0, 0, 0};
     if (s < p.n_seqs) {
       serving_lengths<PAGED>(p, cache, s, q.q0, q.lq, q.k0, q.lk);
-      q.blocks = over_tokens(q.lq + tokens - 1);
+      q.rows = min(q.lq, p.max_q);
+      q.blocks = over_tokens(q.rows + tokens - 1);
     }
     return q;
   };
@@ -143,7 +145,7 @@ __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int 
     if (q.lk <= c * kTileKeys) return 0;
     if (!p.causal) return q.blocks;
     const int y = c * kTileKeys - q.lk + q.lq;   // blocks that end at or before token y see no more
-    return q.blocks - min(over_tokens(max(y, 0)), max(q.blocks - 1, 0));
+    return y >= q.rows ? 0 : q.blocks - over_tokens(max(y, 0));
   };
   auto total = [&](int c) {
     int sum = above(mine, c);
@@ -185,6 +187,7 @@ __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int 
       item.block = __shfl_sync(0xffffffffu, block, src);
       item.q0 = __shfl_sync(0xffffffffu, q.q0, src);
       item.lq = __shfl_sync(0xffffffffu, q.lq, src);
+      item.rows = __shfl_sync(0xffffffffu, q.rows, src);
       item.k0 = __shfl_sync(0xffffffffu, q.k0, src);
       item.lk = __shfl_sync(0xffffffffu, q.lk, src);
       return true;
@@ -291,8 +294,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     const int first = token0 + s * tile_tokens;
-    tiles[s] = found && first < item.lq
-                   ? (keys_seen(p.causal, min(item.lq, first + tile_tokens), item.lq, item.lk) + kTileKeys - 1) / kTileKeys
+    tiles[s] = found && first < item.rows
+                   ? (keys_seen(p.causal, min(item.rows, first + tile_tokens), item.lq, item.lk) + kTileKeys - 1) / kTileKeys
                    : 0;
   }
   const int all = max(tiles[0], tiles[1]);   // stage 1's rows come later: it sees as much, unless it has none
@@ -539,7 +542,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     // ---- softmax ---------------------------------------------------------------------------------
     const int s = warp >> 3, half = (warp >> 2) & 1, token = token0 + s * tile_tokens + in_tile;
     const int h = head * p.group + row - in_tile * p.group;
-    const bool there = work && in_tile < tile_tokens && token < item.lq;
+    const bool there = work && in_tile < tile_tokens && token < item.rows;
     const int limit = there ? keys_seen(p.causal, token + 1, item.lq, item.lk) - key0 : 0;   // keys this row sees from key0 on
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t t_s = lanes + s * kTileKeys + half * kHalfKeys, t_p = lanes + kTmemP + s * kTmemPStage + half * (kHalfKeys / 2);
@@ -778,7 +781,8 @@ __global__ void __launch_bounds__(256) attention_tiles_join_kernel(const Serving
   if (s < 0) return;
   int q0, lq, k0, lk;
   serving_lengths<true>(p, cache, s, q0, lq, k0, lk);
-  const int end = min(lq, ((row - q0) / (2 * tile_tokens) + 1) * 2 * tile_tokens);   // of the row's block
+  if (row - q0 >= p.max_q) return;   // not computed
+  const int end = min(min(lq, p.max_q), ((row - q0) / (2 * tile_tokens) + 1) * 2 * tile_tokens);   // of the row's block
   const int tiles = (keys_seen(p.causal, end, lq, lk) + kTileKeys - 1) / kTileKeys;
   if (tiles <= split.tiles) return;   // written by its CTA
   const int parts = min(split.parts, (tiles + split.tiles - 1) / split.tiles);
@@ -851,9 +855,9 @@ int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, boo
     split.o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kServingCounterBytes);
     split.stats = reinterpret_cast<float2*>(split.o + static_cast<size_t>(split.parts) * p.q_rows * p.heads * p.dim);
   }
-  const int64_t grid = most_blocks(p, 2 * tile_tokens) * p.kv_heads * split.parts;
+  int64_t grid = most_blocks(p, 2 * tile_tokens) * p.kv_heads * split.parts;
   if (grid > 0x7fffffff) return set_error(FB200_INVALID_ARGUMENT, "attention: too many tiles");
-  if (grid == 0) return FB200_OK;
+  if (grid == 0) grid = 1;   // max_q is 0: one CTA looks whether any sequence has rows all the same
   const int spans = p.dim > 64 ? 2 : 1;
   CUtensorMap tq, tk, tv;
   const int64_t qd[4] = {p.dim, p.group, p.q_rows, p.kv_heads}, qs[3] = {p.q_head * 2, p.q_token * 2, p.q_head * p.group * 2};

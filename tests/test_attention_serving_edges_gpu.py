@@ -132,3 +132,51 @@ def test_parts_that_hold_nothing_but_nan_are_not_taken_for_empty(dt, coded):
     assert np.all(np.isnan(got)) and np.all(np.isnan(lse))
 
 
+# ---- more rows than max_q ----------------------------------------------------------------------------
+@pytest.mark.parametrize("h,lq,most,lk", [(4, [3, 1, 2], 1, [50, 20, 300]), (4, [40, 2, 70], 20, [50, 20, 90]),
+                                          (8, [400, 30, 64], 64, [500, 60, 64]), (8, [400, 30, 1], 64, [3000, 1500, 2000]),
+                                          (8, [30, 400], 64, [20, 9000])],
+                         ids=["decode", "one block", "blocks", "parts", "long last"])
+@pytest.mark.parametrize("coded", [False, True], ids=["same", "e4m3"])
+def test_a_sequence_past_max_q_costs_no_other_its_rows(h, lq, most, lk, coded):
+    rng = np.random.default_rng(34)
+    call = Call(rng, BF, h, 2, 64, lq, lk, coded=coded)
+    call.p.max_q = most
+    call.size = capi.attention_paged_workspace(call.p, call.cache)
+    call.work = upload(np.zeros(max(call.size, 1), dtype=np.uint8))
+    if call.size > 4096:                                   # what an earlier call left there
+        call.work.upload(np.concatenate([np.zeros(4096, dtype=np.uint8), np.full(call.size - 4096, 0x41, dtype=np.uint8)]))
+    got, lse = run(call, 322)
+    for s, n in enumerate(lq):
+        rows = slice(call.cu[s], call.cu[s] + min(n, most))
+        k, v = call.pages.values(s, lk[s])
+        o, l, mag, arg = ref.attention(ref.load(call.q[call.cu[s]:call.cu[s + 1]], BF), k, v, np.float32(call.scale), True)
+        tol, tol_l = ref.bounds(o, mag, arg, BF, 64, coded)
+        m = min(n, most)
+        assert np.all(np.abs(got[rows] - o[:m]) <= tol[:m]), s
+        seen = np.isfinite(l[:m])
+        assert np.all(np.isneginf(lse[rows][~seen]))
+        assert np.all(np.abs(lse[rows][seen] - l[:m][seen]) <= (tol_l + 2.0 ** -22 * np.abs(l))[:m][seen])
+        assert np.all(call.got()[call.cu[s] + m:call.cu[s + 1]] == FILL), s       # not computed
+
+
+@pytest.mark.parametrize("most", [64, 100, 0])
+@pytest.mark.parametrize("causal", [1, 0])
+def test_a_prompt_past_max_q_costs_no_other_its_rows(most, causal):
+    rng = np.random.default_rng(35)
+    lq = [700, 33, 100, 1]
+    call = Prompt(rng, BF, 8, 2, 64, lq, causal=causal)
+    call.p.max_q = most
+    got, lse = call.run()
+    assert capi.kernel_status(0) == 322
+    for s, n in enumerate(lq):
+        a, m = call.cu[s], min(n, most)
+        rows = slice(a, a + n)
+        o, l, mag, arg = ref.attention(ref.load(call.q[rows], BF), ref.load(call.k[rows], BF), ref.load(call.v[rows], BF),
+                                       np.float32(call.scale), bool(causal))
+        tol, tol_l = ref.bounds(o, mag, arg, BF, 64)
+        assert np.all(np.abs(ref.load(got[a:a + m], BF) - o[:m]) <= tol[:m]), s
+        assert np.all(np.abs(lse[a:a + m] - l[:m]) <= (tol_l + 2.0 ** -22 * np.abs(l))[:m])
+        assert np.all(got[a + m:a + n] == FILL), s
+
+
