@@ -521,8 +521,14 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
       const int i = r / p.group, h = head * p.group + r - i * p.group;
       const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
       if (lr == 0.0f) x = make_float4(0, 0, 0, 0);
-      T out[4] = {from_f32<T>(x.x * inv), from_f32<T>(x.y * inv), from_f32<T>(x.z * inv), from_f32<T>(x.w * inv)};
-      *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + (q0 + i) * p.o_token + h * p.o_head + d) = *reinterpret_cast<const uint2*>(out);
+      uint2 out;
+      if constexpr (E4M3) {
+        out = make_uint2(pack_finite<T>(x.x * inv, x.y * inv), pack_finite<T>(x.z * inv, x.w * inv));
+      } else {
+        const T four[4] = {from_f32<T>(x.x * inv), from_f32<T>(x.y * inv), from_f32<T>(x.z * inv), from_f32<T>(x.w * inv)};
+        out = *reinterpret_cast<const uint2*>(four);
+      }
+      *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + (q0 + i) * p.o_token + h * p.o_head + d) = out;
       if (d == 0 && p.lse != nullptr) {
         p.lse[static_cast<int64_t>(q0 + i) * p.heads + h] = lr == 0.0f ? -INFINITY : mr * 0.6931471805599453f + logf(lr);
       }

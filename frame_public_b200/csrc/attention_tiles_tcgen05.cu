@@ -100,6 +100,9 @@ template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float lo, floa
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+template <typename T, bool E4M3> __device__ __forceinline__ uint32_t pack_result(float lo, float hi) {
+  return E4M3 ? pack_finite<T>(lo, hi) : pack_pair<T>(lo, hi);
+}
 
 // A CTA's share of the work.
 struct TilesItem {
@@ -732,7 +735,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           uint32_t out[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            out[e] = l == 0.0f ? 0u : pack_pair<T>(__uint_as_float(x[2 * e]) * inv, __uint_as_float(x[2 * e + 1]) * inv);
+            out[e] = l == 0.0f ? 0u : pack_result<T, E4M3>(__uint_as_float(x[2 * e]) * inv, __uint_as_float(x[2 * e + 1]) * inv);
           }
           uint8_t* const to = rows + (i >> 6) * kSpanBytes + row * 128;
           const int chunk = (i >> 3) & 7;
@@ -770,7 +773,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 }
 
 // Joins the parts of split blocks in the order of the keys: one warp per (row, head).
-template <typename T>
+template <typename T, bool E4M3>
 __global__ void __launch_bounds__(256) attention_tiles_join_kernel(const ServingProblem p, const PagedCache cache, const TilesSplit split,
                                                                    int tile_tokens) {
   const int64_t at = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
@@ -812,7 +815,7 @@ __global__ void __launch_bounds__(256) attention_tiles_join_kernel(const Serving
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   if (mine) {
-    const uint2 out = l == 0.0f ? make_uint2(0, 0) : make_uint2(pack_pair<T>(sum.x * inv, sum.y * inv), pack_pair<T>(sum.z * inv, sum.w * inv));
+    const uint2 out = l == 0.0f ? make_uint2(0, 0) : make_uint2(pack_result<T, E4M3>(sum.x * inv, sum.y * inv), pack_result<T, E4M3>(sum.z * inv, sum.w * inv));
     *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + static_cast<int64_t>(row) * p.o_token + h * p.o_head + lane * 4) = out;
   }
   if (lane == 0 && p.lse != nullptr) p.lse[at] = l == 0.0f ? -INFINITY : m * 0.6931471805599453f + logf(l);
@@ -904,8 +907,9 @@ int launch_attention_tiles(const ServingProblem& p, const PagedCache* cache, boo
   if (int rc = after_launch("attention_tiles_kernel")) return rc;
   if (split.parts == 1) return FB200_OK;
   const int64_t joins = (static_cast<int64_t>(p.q_rows) * p.heads + 7) / 8;
-  if (p.dtype == FB200_BF16) attention_tiles_join_kernel<__nv_bfloat16><<<static_cast<unsigned>(joins), 256, 0, stream>>>(p, view, split, tile_tokens);
-  else attention_tiles_join_kernel<__half><<<static_cast<unsigned>(joins), 256, 0, stream>>>(p, view, split, tile_tokens);
+  auto join = [&](auto kernel) { kernel<<<static_cast<unsigned>(joins), 256, 0, stream>>>(p, view, split, tile_tokens); };
+  if (p.dtype == FB200_BF16) e4m3 ? join(attention_tiles_join_kernel<__nv_bfloat16, true>) : join(attention_tiles_join_kernel<__nv_bfloat16, false>);
+  else e4m3 ? join(attention_tiles_join_kernel<__half, true>) : join(attention_tiles_join_kernel<__half, false>);
   return after_launch("attention_tiles_join_kernel");
 }
 

@@ -6,7 +6,7 @@
 // A power of two keeps every product exact, so the codes do not depend on how the division is done,
 // and code * 2^e is exact in bfloat16 when it is read.  A relative step of 2^-4 is all e4m3 has either
 // way; the scale only has to keep small numbers out of its denormals.
-// Read: code * 2^e, rounded once.
+// Read: code * 2^e, rounded once, at most the type's largest finite number.
 // Both are bound by HBM: (2 + 1) bytes a number either way, 1/head_dim more for the scales.  A lane group
 // (16 bytes a lane on the dense side) takes four heads of one token: the token's place, a binary search and two
 // dependent loads, is found once for eight vectors in flight (one head a group: TIME_BEFORE).
@@ -174,16 +174,15 @@ __global__ void __launch_bounds__(256) kv_cache_write_kernel(PagedCache cache, D
   }
 }
 
-// Eight codes times the row's scale, rounded once to T.
+// Eight codes times the row's scale, rounded once to T (at most its largest finite number).
 template <typename T> __device__ __forceinline__ uint4 decode8(uint2 codes, float scale) {
-  T out[8];
+  uint32_t out[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = e4m3x2_to_f32(((i < 2 ? codes.x : codes.y) >> ((i & 1) * 16)) & 0xFFFFu);
-    out[2 * i] = from_f32<T>(f.x * scale);
-    out[2 * i + 1] = from_f32<T>(f.y * scale);
+    out[i] = pack_finite<T>(f.x * scale, f.y * scale);
   }
-  return *reinterpret_cast<const uint4*>(out);
+  return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
 template <typename T, bool E4M3, int LANES, int HEADS>

@@ -9,6 +9,8 @@
 
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace fb200 {
@@ -95,6 +97,16 @@ __host__ __device__ inline uint32_t scale_byte_of(uint32_t amax_bits) {
 }
 // 2^(b - 127); 255 is a NaN, b = 0 (never written) reads as 0.
 __device__ __forceinline__ float scale_of_byte(uint32_t b) { return __uint_as_float(b == 255u ? 0x7FC00000u : b << 23); }
+
+// The largest number of a row may round up to 256 * 2^e, which at the very top of T's range is past its largest
+// finite number (65504 becomes 65536 in float16, 248 * 2^120 and more 2^128 in bfloat16).  What comes out of an
+// e4m3 cache stops at that number, so that finite numbers stay finite; NaN stays NaN.  Two numbers, `lo` first.
+template <typename T> __device__ __forceinline__ uint32_t pack_finite(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 
 __device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t pair) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3);

@@ -441,7 +441,8 @@ typedef struct fb200_attention_params {
 /* A paged cache: token t of a sequence lies in page block_table[s][t / page_size], at place
  * t % page_size.  k and v share the strides (elements of `dtype`).  dtype: BF16 / F16, or U8 for
  * e4m3 codes with one scale per (token, kv head): byte b stands for 2^(b - 127), and the values are
- * code * 2^(b - 127); b = 255 makes the whole token-head NaN.  page_size a power of two from 8 up. */
+ * code * 2^(b - 127); b = 255 makes the whole token-head NaN.  What attention computes from finite
+ * e4m3 values stops at the largest finite number of its type.  page_size a power of two from 8 up. */
 typedef struct fb200_kv_cache {
   void* k;
   void* v;
@@ -473,7 +474,9 @@ FB200_API int fb200_kv_cache_write(const fb200_kv_cache* cache, const void* k, i
                                    int64_t rows, int dtype, fb200_stream stream);
 /* The first cu_kv[s+1] - cu_kv[s] cached tokens of every sequence as rows cu_kv[s] .. of dense k and
  * v ([rows, kv_heads, head_dim] of `dtype`).  e4m3 values are exact in bfloat16 and rounded once to
- * float16.  Bad pages as in the write (their rows stay as they were). */
+ * float16; a value past the type's largest finite number (the largest number of a row may have been
+ * rounded up at the write) becomes that number.  Bad pages as in the write (their rows stay as they
+ * were). */
 FB200_API int fb200_kv_cache_read(const fb200_kv_cache* cache, void* k, int64_t k_token_stride,
                                   int64_t k_head_stride, void* v, int64_t v_token_stride,
                                   int64_t v_head_stride, const int32_t* cu_kv, const int32_t* block_table,

@@ -180,3 +180,50 @@ def test_a_prompt_past_max_q_costs_no_other_its_rows(most, causal):
         assert np.all(got[a + m:a + n] == FILL), s
 
 
+# ---- the ends of the types ---------------------------------------------------------------------------
+TOP = {BF: 2.0 ** 128 - 2.0 ** 120, FH: 65504.0}
+
+
+def finite_values(pages, seq, n, dt):
+    """What an e4m3 cache's finite numbers read as: rounded to the type, the largest finite number at most."""
+    return [np.where(np.isnan(x), x, np.clip(x, -TOP[dt], TOP[dt])) for x in pages.values(seq, n)]
+
+
+@pytest.mark.parametrize("dt", [BF, FH])
+def test_finite_numbers_at_the_top_of_the_type_read_back_finite(dt):
+    """A row's largest number may round up to 256 * 2^e, which is past the 16-bit type at its very top."""
+    rng = np.random.default_rng(36)
+    h, hk, d, n = 4, 2, 64, 40
+    call = Call(rng, dt, h, hk, d, [1], [n], coded=True)
+    x = ref.store(rng.uniform(0.9, 1.0, (n, hk, d)) * rng.choice([-1.0, 1.0], (n, hk, d)) * TOP[dt], dt)
+    x[3, 0, :2] = ref.store(np.array([TOP[dt], -TOP[dt]]), dt)
+    x[4, 1] = 0x7F80 if dt == BF else 0x7C00                # an infinity reads as NaN
+    call.pages.put(0, 0, x, x)
+    resend(call)
+    outs, cu = [upload(np.full((n, hk, d), FILL, dtype=np.uint16)) for _ in range(2)], upload(np.array([0, n], dtype=np.int32))
+    capi.kv_cache_read(call.cache, outs[0].ptr, hk * d, d, outs[1].ptr, hk * d, d, cu.ptr, call.pages.dev["table"].ptr,
+                       call.pages.table.shape[1], 1, n, dt)
+    capi.synchronize()
+    assert np.abs(np.nan_to_num(call.pages.values(0, n)[0])).max() > TOP[dt]     # the case it is about
+    for out, want in zip(outs, finite_values(call.pages, 0, n, dt)):
+        got = ref.load(out.download(np.uint16, (n, hk, d)), dt)
+        assert np.array_equal(np.isnan(got), np.isnan(want)) and np.all(np.isnan(want[4, 1]))
+        fine = ~np.isnan(want)
+        assert np.array_equal(got[fine], ref.load(ref.store(want, dt), dt)[fine])
+
+
+@pytest.mark.parametrize("lq,n", [(1, 40), (20, 40), (20, 3000)], ids=["decode", "chunk", "parts"])
+@pytest.mark.parametrize("dt", [BF, FH])
+def test_attention_over_e4m3_values_at_the_top_of_the_type_stays_finite(dt, lq, n):
+    """All values equal the largest finite number, so every row does, whatever the weights."""
+    rng = np.random.default_rng(37)
+    call = Call(rng, dt, 8, 2, 64, [lq], [n], coded=True)
+    k = ref.store(rng.standard_normal((n, 2, 64)), dt)
+    call.pages.put(0, 0, k, ref.store(np.full((n, 2, 64), TOP[dt]), dt))
+    resend(call)
+    got, lse = run(call)
+    assert np.all(np.isfinite(got)) and np.all(np.isfinite(lse))
+    unit = ref.UNIT[dt]
+    assert np.all(got >= TOP[dt] * (1 - 2 * unit))
+
+
