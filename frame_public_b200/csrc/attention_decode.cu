@@ -427,7 +427,7 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
           }
         }
       }
-      const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+      const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0] - kProbLift<M>, m[1] == -INFINITY ? 0.0f : m[1] - kProbLift<M>};
       uint32_t pa[kKeyTiles / 2][4] = {};   // P as A operands of 16 keys each
 #pragma unroll
       for (int n = 0; n < kKeyTiles; ++n) {
@@ -530,7 +530,7 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
       }
       *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + (q0 + i) * p.o_token + h * p.o_head + d) = out;
       if (d == 0 && p.lse != nullptr) {
-        p.lse[static_cast<int64_t>(q0 + i) * p.heads + h] = lr == 0.0f ? -INFINITY : mr * 0.6931471805599453f + logf(lr);
+        p.lse[static_cast<int64_t>(q0 + i) * p.heads + h] = lr == 0.0f ? -INFINITY : (mr - kProbLift<M>) * 0.6931471805599453f + logf(lr);
       }
     };
     for (int r0 = 0; r0 < rows; r0 += kDecodeJoinRows) {

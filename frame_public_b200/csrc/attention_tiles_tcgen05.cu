@@ -20,8 +20,8 @@
 // tile are computed as soon as the threads have read those of this one.  Above: S0, S1, O0, O1 (128 each)
 // leave no room, P lies over S, and the next scores follow P V; P is handed over in halves so that only
 // the second half of P V lies between the two.
-// O is only rescaled when a row's maximum grew by more than 2^8 since the last time (the exponents stay
-// below 2^8 then, which fp32 sums and 16-bit P hold as well as values up to 1).
+// O is only rescaled when a row's maximum grew by more than 2^8 since the last time (P stays below 2^8 then,
+// float16 P, which is taken times 2^7, below 2^15: fp32 sums and the 16-bit types hold that).
 //
 // Bounds: 4 * pairs * head_dim FLOP against the tensor pipe; one exponential per pair against the
 // XU pipe (16 per SM and cycle: 1024 cycles for a 128 x 128 tile whose two products take 512 to 1024).
@@ -676,7 +676,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           tmem_st_32x32b_x16(t_o + i, x);
         }
       }
-      const float mc = m == -INFINITY ? 0.0f : m * to_exp;
+      const float mc = m == -INFINITY ? 0.0f : m * to_exp - kProbLift<M>;
       float2 sum = make_float2(0.0f, 0.0f);
       const float2 c2 = make_float2(c, c), nm2 = make_float2(-mc, -mc);
 #pragma unroll
@@ -759,8 +759,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         }
       }
       if (there && half == 0) {
-        if (parted) split.stats[part * static_cast<int64_t>(p.q_rows) * p.heads + at] = make_float2(any ? m * to_exp : -INFINITY, l);
-        else if (p.lse != nullptr) p.lse[at] = l == 0.0f ? -INFINITY : m * to_exp * 0.6931471805599453f + logf(l);
+        if (parted) split.stats[part * static_cast<int64_t>(p.q_rows) * p.heads + at] = make_float2(any ? m * to_exp - kProbLift<M> : -INFINITY, l);
+        else if (p.lse != nullptr) p.lse[at] = l == 0.0f ? -INFINITY : (m * to_exp - kProbLift<M>) * 0.6931471805599453f + logf(l);
       }
     }
   }

@@ -138,10 +138,15 @@ __device__ __forceinline__ float query_lift(float amax, float& factor) {
   factor = __uint_as_float(static_cast<uint32_t>(127 + up1) << 23);
   return __uint_as_float(static_cast<uint32_t>(127 - up1) << 23);
 }
+// float16 holds nothing below 2^-24, and a row over a long cache can have most of its weight in keys far below the
+// largest.  So float16 probabilities are taken times 2^7: with the 2^8 by which the running maximum may lag they
+// stay below 65504, and a weight is lost from 2^-32 of the row's largest down.  bfloat16 has the range of fp32.
+template <typename M> constexpr float kProbLift = std::is_same<M, __half>::value ? 7.0f : 0.0f;
+
 // A probability times its value's scale 2^e has to fit float16 too, so rows are normalised by the largest
 // 2^(score + e) instead of 2^score.  e below a floor counts as the floor (rows of zeros have e = -126), and so
 // does that of a row that is not finite, which makes NaN of the result through its scale.  The row sum is then
-// down to 2^-e of its largest term: above e = 100 (values past 10^32) terms 2^-26 of it start to be lost.
+// down to 2^(7 - e) of its largest term: above e = 107 (values past 10^34) terms 2^-26 of it start to be lost.
 constexpr int kScaleFloor = -60;
 __device__ __forceinline__ float scale_exponent(uint32_t b) {
   const int e = b == 255u ? kScaleFloor : static_cast<int>(b) - 127;

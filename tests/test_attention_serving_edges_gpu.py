@@ -227,3 +227,80 @@ def test_attention_over_e4m3_values_at_the_top_of_the_type_stays_finite(dt, lq, 
     assert np.all(got >= TOP[dt] * (1 - 2 * unit))
 
 
+def score_error(arg, d):
+    return (d + 8) * 2.0 ** -23 * arg + 2.0 ** -20
+
+
+def small_weights_bound(o, mag, arg, dt, d, n, weights, values):
+    """Probabilities are held in float16 for float16 and e4m3 caches, the largest as 2^7 or more: half a step
+    is 2^-11 of a probability, and at least 2^-25, which is 2^-32 of the row's largest weight.  (`weights`:
+    that largest one per row, p times the value's scale; `values`: the sum over the keys of what it is
+    multiplied with, codes or numbers.)  A score is an fp32 sum of d products, as in ref.bounds; O and the row
+    sum grow in fp32 by 16 keys at a time or more, each addition truncated at worst."""
+    delta, steps = score_error(arg, d), n / 16 * 2.0 ** -23
+    return (2.0 ** -11 + 2 * delta[..., None] + 2 * steps) * mag + ref.UNIT[dt] * np.abs(o) + 2.0 ** -24 + 2.0 ** -32 * weights * values
+
+
+@pytest.mark.parametrize("form,dt,coded", [("prompt", FH, False)] +
+                         [(f, dt, c) for f in ("decode", "draft", "chunk") for dt, c in ((FH, False), (BF, True), (FH, True))])
+def test_many_small_probabilities_beside_a_large_one_are_not_lost(form, dt, coded):
+    """One key outweighs each of 2^17 others by 2^26, and in all columns but one their values are 2^10 as large:
+    together the others make most of the result.  Over a cache so many sequences share the pages that one CTA
+    walks all keys of a sequence."""
+    rng = np.random.default_rng(38)
+    h, hk, d, n = 2, 1, 64, 1 << 17
+    copies, lq = {"decode": (300, 1), "draft": (300, 6), "chunk": (150, 20), "prompt": (1, 20)}[form]
+    scale = 0.125
+    q = ref.store(np.full((lq, h, d), 1.5), dt)
+    k = np.zeros((n, hk, d))
+    k[7] = 1.5                                              # 2.25 * 64 / 8 = 18 = 25.97 in powers of two
+    v = np.full((n, hk, d), 8.0) * rng.choice([0.875, 1.0, 1.125], (n, hk, d))
+    v[7] = 2.0 ** -7
+    v[7, :, 0] = 8.0                                        # its scale is the others'
+    k, v = ref.store(k, dt), ref.store(v, dt)
+    e = np.zeros(n)
+    if form == "prompt":
+        got, lse = Prompt(rng, dt, h, hk, d, [lq], [n], scale, 0, q, k, v).run()
+        kk, vv = ref.load(k, dt), ref.load(v, dt)
+    else:
+        pages = ref.Pages(rng, [n], 128, hk, d, dt, coded, True)
+        pages.put(0, 0, k, v)
+        cache, table = pages.upload(), upload(np.repeat(pages.table, copies, 0))
+        p = params(dt, h, hk, d, [lq] * copies, [n], lq * copies, 0, scale)
+        size = capi.attention_paged_workspace(p, cache)
+        work, dq = upload(np.zeros(max(size, 1), dtype=np.uint8)), upload(np.tile(q, (copies, 1, 1)))
+        out, dlse = upload(np.full((lq * copies, h, d), FILL, dtype=np.uint16)), capi.DeviceBuffer(lq * copies * h * 4)
+        dcu, dlen = upload(ref.offsets([lq] * copies)), upload(np.full(copies, n, dtype=np.int32))
+        capi.attention_paged(p, cache, dq.ptr, out.ptr, dcu.ptr, dlen.ptr, table.ptr, pages.table.shape[1], work.ptr, size, lse=dlse.ptr)
+        capi.synchronize()
+        got = out.download(np.uint16, (copies, lq, h, d))
+        lse = dlse.download(np.float32, (copies, lq, h)).astype(np.float64)
+        kk, vv = pages.values(0, n)
+        if coded:
+            e = np.maximum(pages.vs[pages._at(pages.vs, 0, np.arange(n))][:, 0].astype(np.float64) - 127, -60)
+    assert capi.kernel_status(0) == 0
+    got = ref.load(got, dt)
+    o, l, mag, arg = ref.attention(ref.load(q, dt), kk, vv, scale, False)
+    p = np.exp(ref.load(q, dt)[0, 0] @ kk[:, 0].T * scale - l[0, 0])
+    tol = small_weights_bound(o, mag, arg, dt, d, n, np.max(p * 2.0 ** e), (np.abs(vv[:, 0]) * 2.0 ** -e[:, None]).sum(0))
+    assert np.all(tol < 0.1 * np.abs(o))                    # the bound says something
+    assert np.all(np.abs(got - o) <= tol), float(np.max(np.abs(got - o) / tol))
+    assert np.all(np.abs(lse - l) <= score_error(arg, d) + 2.0 ** -21 + 2.0 ** -22 * np.abs(l) + n / 16 * 2.0 ** -23)
+
+
+@pytest.mark.parametrize("lq", [1, 3, 20], ids=["decode", "draft", "chunk"])
+@pytest.mark.parametrize("dt,d", [(BF, 64), (FH, 128)])
+def test_probabilities_over_an_e4m3_cache_keep_the_bits_of_float16(dt, d, lq):
+    """Ordinary numbers, held to half a step of float16 in P (serving_ref's bound allows bfloat16's)."""
+    rng = np.random.default_rng(45)
+    n, h, hk = 500, 8, 2
+    call = Call(rng, dt, h, hk, d, [lq], [n], coded=True)
+    got, lse = run(call)
+    kk, vv = call.pages.values(0, n)
+    o, l, mag, arg = ref.attention(ref.load(call.q, dt), kk, vv, np.float32(call.scale), True)
+    e = call.pages.vs[call.pages._at(call.pages.vs, 0, np.arange(n))].astype(np.float64) - 127      # [n, hk]
+    codes = (np.abs(vv) * 2.0 ** -e[..., None]).sum(0).repeat(h // hk, 0)                           # [h, d]
+    tol = small_weights_bound(o, mag, arg, dt, d, n, 2.0 ** e.max(), codes)
+    assert np.all(np.abs(got - o) <= tol), float(np.max(np.abs(got - o) / tol))
+
+
