@@ -127,16 +127,15 @@ __device__ __forceinline__ uint32_t codes_high(uint32_t w) {
 }
 // What the codes of a cache are multiplied with is float16 as well.  A bfloat16 query row is brought there by
 // the power of two that puts its largest magnitude into [2^14, 2^15): products with a power of two are exact,
-// and what falls below float16's smallest step (2^-24) is 2^-38 of that magnitude.  Returns the inverse's
-// exponent as a factor for the scores.
+// and what falls below float16's smallest step (2^-24) is 2^-38 of that magnitude.  No power above 2^120 is
+// taken, whose inverse fp32 holds well: every bfloat16 is a multiple of 2^-133, so what it is multiplied with
+// 2^120 is one of 2^-13, and rows too small to reach 2^14 lose nothing.  Returns the inverse as a factor for
+// the scores.
 __device__ __forceinline__ float query_lift(float amax, float& factor) {
-  const uint32_t e = __float_as_uint(amax) >> 23;   // biased; 0 and 255 (nothing, infinity, NaN) stay as they are
-  const bool plain = e >= 1u && e <= 254u;
-  // 2^(14 + 127 - e) from 2^-113 to 2^140: in two steps where one would leave fp32
-  const int up = plain ? 141 - static_cast<int>(e) : 0;
-  const int up1 = up > 120 ? 120 : up;
-  factor = __uint_as_float(static_cast<uint32_t>(127 + up1) << 23);
-  return __uint_as_float(static_cast<uint32_t>(127 - up1) << 23);
+  const int e = static_cast<int>(__float_as_uint(amax) >> 23);   // biased; 0: subnormal or nothing, 255: not finite
+  const int up = e == 255 ? 0 : min(141 - e, 120);               // 2^(14 + 127 - e), from 2^-113 on
+  factor = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+  return __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
 }
 // float16 holds nothing below 2^-24, and a row over a long cache can have most of its weight in keys far below the
 // largest.  So float16 probabilities are taken times 2^7: with the 2^8 by which the running maximum may lag they

@@ -304,3 +304,21 @@ def test_probabilities_over_an_e4m3_cache_keep_the_bits_of_float16(dt, d, lq):
     assert np.all(np.abs(got - o) <= tol), float(np.max(np.abs(got - o) / tol))
 
 
+@pytest.mark.parametrize("lq,n", [(1, 100), (20, 100)], ids=["decode", "chunk"])
+@pytest.mark.parametrize("top", [2.0 ** -126, 2.0 ** -127, 2.0 ** -131])
+def test_the_smallest_bfloat16_queries_over_an_e4m3_cache(lq, n, top):
+    """Query rows below or near the smallest normal number, keys near the largest: scores of a few units."""
+    rng = np.random.default_rng(39)
+    h, hk, d, dt = 8, 2, 64, BF
+    call = Call(rng, dt, h, hk, d, [lq], [n], coded=True)
+    q = np.round(rng.uniform(-1, 1, (lq, h, d)) * top / 2.0 ** -133) * 2.0 ** -133
+    q[..., 0] = top                                         # multiples of the smallest subnormal number
+    call.q = ref.store(q, dt)
+    assert np.array_equal(ref.load(call.q, dt), q)
+    call.scale = call.p.scale = 2.0 ** -126 / top
+    call.pages.put(0, 0, ref.store(rng.standard_normal((n, hk, d)) * 2.0 ** 124, dt), ref.store(rng.standard_normal((n, hk, d)), dt))
+    resend(call)
+    got, lse = run(call)
+    near(got, lse, call.q, *call.pages.values(0, n), dt, d, call.scale, True)
+
+
