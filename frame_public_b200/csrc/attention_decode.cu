@@ -159,6 +159,7 @@ attention_decode_kernel(const ServingProblem p, const PagedCache cache, uint8_t*
     for (int s = lane; s < p.n_seqs; s += 32) {
       int lk;
       sum += pair_tiles<kTile>(p, cache, s, lk);
+      if (blockIdx.x == 0 && warp == 0 && !lengths_fit<true>(p.cu_q, p.kv_len, s, p.q_rows, most_cached(cache.table_stride, cache.page_shift))) record_fault(status, kFaultBadLength);
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);

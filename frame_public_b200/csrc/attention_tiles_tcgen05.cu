@@ -121,7 +121,7 @@ __device__ __forceinline__ int keys_seen(int causal, int end, int lq, int lk) {
 // one with more rows takes no other's place in the grid.  Run by one warp; returns false past the last item.
 template <bool PAGED>
 __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int rank, int tokens, uint32_t tokens_inverse,
-                          TilesItem& item, int* status) {
+                          TilesItem& item) {
   const int lane = threadIdx.x & 31;
   // y / tokens for 0 <= y < 2^31: tokens_inverse = floor(2^32 / tokens) gives it or one less
   auto over_tokens = [&](int y) {
@@ -155,13 +155,8 @@ __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int 
     for (int s = lane + 32; s < p.n_seqs; s += 32) sum += above(load(s), c);
     return __reduce_add_sync(0xffffffffu, sum);
   };
-  int most = mine.lk, widest = mine.lq;
-  for (int s = lane + 32; s < p.n_seqs; s += 32) {
-    const Seq q = load(s);
-    most = max(most, q.lk);
-    widest = max(widest, q.lq);
-  }
-  if (rank == 0 && widest > p.max_q) record_fault(status, kFaultBadLength);
+  int most = mine.lk;
+  for (int s = lane + 32; s < p.n_seqs; s += 32) most = max(most, load(s).lk);
   const int longest = __reduce_max_sync(0xffffffffu, most);
   if (rank >= total(-1)) return false;
   int lo = -1, hi = (longest + kTileKeys - 1) / kTileKeys;   // total(lo) > rank >= total(hi)
@@ -198,6 +193,15 @@ __device__ bool find_item(const ServingProblem& p, const PagedCache& cache, int 
     left -= __shfl_sync(0xffffffffu, upto, 31);
   }
   return false;
+}
+
+// Records sequences that are cut.  Run by one warp of the call, out of line: inlined it took registers from the
+// loops over the tiles (2 x 8192 538 -> 547 us, e4m3 chunks of float16 405 -> 421).
+template <bool PAGED>
+__device__ __noinline__ void check_lengths(const int32_t* cu_q, const int32_t* keys, int n_seqs, int q_rows, int most_keys, int max_q, int* status) {
+  for (int s = threadIdx.x & 31; s < n_seqs; s += 32) {
+    if (!lengths_fit<PAGED>(cu_q, keys, s, q_rows, most_keys) || cu_q[s + 1] - cu_q[s] > max_q) record_fault(status, kFaultBadLength);
+  }
 }
 
 // Barriers, the swap of row maxima and an e4m3 cache's scales, in front of the tiles.
@@ -258,7 +262,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   const int row = threadIdx.x & 127, in_tile = row / p.group;
   if (warp == 0) {
     TilesItem it;
-    const bool found = find_item<PAGED>(p, cache, pair / p.kv_heads, 2 * tile_tokens, tokens_inverse, it, status);
+    const bool found = find_item<PAGED>(p, cache, pair / p.kv_heads, 2 * tile_tokens, tokens_inverse, it);
     if (lane == 0) {
       if (found) *item_ptr = it;
       *found_ptr = found;
@@ -353,6 +357,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
         }
       }
+    }
+    if (blockIdx.x == 0) {   // here it delays nothing: the last copies are on their way
+      check_lengths<PAGED>(p.cu_q, PAGED ? p.kv_len : p.cu_kv, p.n_seqs, p.q_rows, PAGED ? most_cached(cache.table_stride, cache.page_shift) : p.kv_rows, p.max_q, status);
     }
     __syncwarp();
   } else if (E4M3 && warp >= kCodeWarp) {

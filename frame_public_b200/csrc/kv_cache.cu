@@ -146,6 +146,7 @@ __global__ void __launch_bounds__(256) kv_cache_write_kernel(PagedCache cache, D
   }
   const int seq = u.heads > 0 ? sequence_of_row(cu_q, n_seqs, u.row) : -1;
   const int64_t pos = seq >= 0 ? static_cast<int64_t>(kv_len[seq]) - cu_q[seq + 1] + u.row : 0;
+  if (seq >= 0 && !span_fits(cu_q, seq, rows)) record_fault(status, kFaultBadLength);
   const int page = seq >= 0 ? place_of(cache, seq, pos, status) : -1;
   constexpr int kBytes = E4M3 ? 1 : 2;
   const int64_t at = page >= 0 ? token_offset(cache, page, static_cast<int>(pos), u.head) * kBytes : 0;
@@ -193,6 +194,7 @@ __global__ void __launch_bounds__(256) kv_cache_read_kernel(PagedCache cache, De
   if (u.heads == 0 || lane >= lanes) return;
   const int seq = sequence_of_row(cu_kv, n_seqs, u.row);
   if (seq < 0) return;
+  if (!span_fits(cu_kv, seq, rows)) record_fault(status, kFaultBadLength);
   const int64_t pos = static_cast<int64_t>(u.row) - cu_kv[seq];
   const int page = place_of(cache, seq, pos, status);
   if (page < 0) return;

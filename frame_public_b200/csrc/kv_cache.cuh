@@ -4,7 +4,7 @@
 //
 // Lengths and page numbers live on the device, so a kernel cannot trust them: every offset is cut to
 // the extents the host gave, a page number outside the cache becomes page 0, and the status word
-// records it.  No value of cu_q, kv_len or the block table makes an access out of range.
+// records either.  No value of cu_q, kv_len or the block table makes an access out of range.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -17,7 +17,7 @@ namespace fb200 {
 
 enum ServingFault : int {
   kFaultBadPage = 321,     // a page number outside the cache
-  kFaultBadLength = 322,   // a token outside the block table, or more query rows than max_q
+  kFaultBadLength = 322,   // an offset or a length outside the extents, or more query rows than max_q
 };
 
 constexpr int64_t kMostTokens = int64_t(1) << 30;   // of a packed tensor or a cached sequence: sums of a few stay in 32 bits
@@ -31,6 +31,11 @@ __host__ __device__ inline void sequence_span(const int32_t* cu, int64_t s, int6
   const int64_t b = clamp_i64(cu[s], 0, rows), e = clamp_i64(cu[s + 1], b, rows);
   begin = static_cast<int>(b);
   len = static_cast<int>(e - b);
+}
+
+// Whether sequence_span takes the bounds of sequence s as they are.
+__host__ __device__ inline bool span_fits(const int32_t* cu, int64_t s, int64_t rows) {
+  return cu[s] >= 0 && cu[s] <= cu[s + 1] && cu[s + 1] <= rows;
 }
 
 // The sequence that owns packed row `row`, or -1.  cu does not decrease; whatever it holds, the search
@@ -72,9 +77,12 @@ __device__ __forceinline__ int page_number(const PagedCache& c, int64_t s, int64
 }
 
 // Cached tokens of a sequence, cut to what its table row can hold.
-__host__ __device__ inline int cached_length(int32_t kv_len, int64_t table_stride, int page_shift) {
+__host__ __device__ inline int most_cached(int64_t table_stride, int page_shift) {
   const int64_t most = table_stride << page_shift;
-  return static_cast<int>(clamp_i64(kv_len, 0, most < kMostTokens ? most : kMostTokens));
+  return static_cast<int>(most < kMostTokens ? most : kMostTokens);
+}
+__host__ __device__ inline int cached_length(int32_t kv_len, int64_t table_stride, int page_shift) {
+  return static_cast<int>(clamp_i64(kv_len, 0, most_cached(table_stride, page_shift)));
 }
 
 __device__ __forceinline__ int64_t token_offset(const PagedCache& c, int page, int token, int head) {

@@ -425,7 +425,8 @@ FB200_API int fb200_attention_fan(const void* q_base, int64_t q_rows, int64_t q_
  * every stride a multiple of 8 elements (16 for e4m3 codes).  dtype BF16 or F16; head_dim a
  * multiple of 16 up to 128; heads a multiple of kv_heads, heads / kv_heads <= 64.  Anything else
  * is FB200_UNIMPLEMENTED or FB200_INVALID_ARGUMENT.  q_rows and the other extents bound every access:
- * offsets and lengths that leave them are cut to them.  All pointers belong to the current device. */
+ * offsets and lengths that leave them (negative, falling, past the rows or the table) are cut to them and
+ * recorded as kernel status 322.  All pointers belong to the current device. */
 typedef struct fb200_attention_params {
   int64_t n_seqs, heads, kv_heads, head_dim;
   int64_t q_rows;    /* rows of q and o */
@@ -465,7 +466,8 @@ FB200_API int fb200_attention_prompt(const fb200_attention_params* params, const
  * and head, the smallest 2^e with e >= -126 and max|x| <= 448 * 2^e, and x * 2^-e rounded to nearest
  * even; a token-head with an infinity or a NaN is stored as scale byte 255 and codes 0.  block_table:
  * device int32 [n_seqs, table_stride].  A page number outside the cache, or a token outside the
- * table, is skipped and recorded as kernel status 321 / 322.  Two tokens of one call must not share
+ * table, is skipped and recorded as kernel status 321 / 322, offsets of a stored row's sequence that leave
+ * the rows as 322 too.  Two tokens of one call must not share
  * a place (pages shared by sequences hold whole prefixes, which are not written again). */
 FB200_API int fb200_kv_cache_write(const fb200_kv_cache* cache, const void* k, int64_t k_token_stride,
                                    int64_t k_head_stride, const void* v, int64_t v_token_stride,

@@ -322,3 +322,74 @@ def test_the_smallest_bfloat16_queries_over_an_e4m3_cache(lq, n, top):
     near(got, lse, call.q, *call.pages.values(0, n), dt, d, call.scale, True)
 
 
+# ---- lengths that leave the extents ------------------------------------------------------------------
+@pytest.mark.parametrize("lq", [[1, 1], [20, 30]], ids=["decode", "chunk"])
+@pytest.mark.parametrize("what,cu,lens", [("past the table", None, [300, 1 << 20]), ("negative", None, [-3, 200]),
+                                          ("past the rows", [0, 1, 1 << 28], None), ("before the rows", [-5, 1, 2], None),
+                                          ("falling", [0, 2, 1], None), ("nothing left", [9, 9, 3], None)])
+def test_lengths_that_are_cut_are_recorded(lq, what, cu, lens):
+    """The rows are those of the lengths that remain (the second sequence's table row holds its 200 tokens)."""
+    rng = np.random.default_rng(40)
+    call = Call(rng, BF, 8, 2, 64, lq, [208, 208])
+    if cu is not None:
+        call.dcu.upload(np.array(cu, dtype=np.int32))
+    if lens is not None:
+        call.dlen.upload(np.array(lens, dtype=np.int32))
+    run(call, 322)
+    if lens is None:
+        return
+    lk = [max(0, min(n, 208)) for n in lens]
+    seqs = [tuple(call.pages.values(s, n)) for s, n in enumerate(lk)]
+    check_rows(call.got(), call.lse.download(np.float32, call.q.shape[:2]).astype(np.float64), call.q, call.cu, seqs, BF, 64,
+               np.float32(call.scale), 1)
+
+
+@pytest.mark.parametrize("cu,cuk", [([0, 40, 1 << 28], None), ([-1, 40, 70], None), (None, [0, 40, 71]), (None, [0, 60, 40])])
+def test_prompt_offsets_that_are_cut_are_recorded(cu, cuk):
+    rng = np.random.default_rng(41)
+    call = Prompt(rng, BF, 4, 2, 64, [40, 30])
+    if cu is not None:
+        call.dcu.upload(np.array(cu, dtype=np.int32))
+    if cuk is not None:
+        call.dcuk.upload(np.array(cuk, dtype=np.int32))
+    call.run()
+    assert capi.kernel_status(0) == 322
+    call = Prompt(rng, BF, 4, 2, 64, [40, 30])
+    call.run()
+    assert capi.kernel_status(0) == 0
+
+
+@pytest.mark.parametrize("cu", [[0, 3, 9], [-2, 3, 5]])
+@pytest.mark.parametrize("coded", [False, True], ids=["same", "e4m3"])
+def test_cache_offsets_that_leave_the_rows_are_recorded(cu, coded):
+    rng = np.random.default_rng(42)
+    hk, d = 2, 64
+    pages = ref.Pages(rng, [20, 20], 16, hk, d, BF, coded, True)
+    cache = pages.upload()
+    x, dcu = upload(ref.store(rng.standard_normal((5, hk, d)), BF)), upload(np.array(cu, dtype=np.int32))
+    lens = upload(np.array([20, 20], dtype=np.int32))
+    table, stride = pages.dev["table"].ptr, pages.table.shape[1]
+    capi.kv_cache_write(cache, x.ptr, hk * d, d, x.ptr, hk * d, d, dcu.ptr, lens.ptr, table, stride, 2, 5, BF)
+    capi.synchronize()
+    assert capi.kernel_status(0) == 322
+    capi.kv_cache_read(cache, x.ptr, hk * d, d, x.ptr, hk * d, d, dcu.ptr, table, stride, 2, 5, BF)
+    capi.synchronize()
+    assert capi.kernel_status(0) == 322
+
+
+def test_tokens_without_a_place_are_not_stored():
+    """More new tokens than the length counts: the first ones would lie before the sequence."""
+    rng = np.random.default_rng(43)
+    hk, d, page, dt = 2, 64, 16, BF
+    pages = ref.Pages(rng, [40], page, hk, d, dt, False, True, fill=7)
+    cache = pages.upload()
+    x = ref.store(rng.standard_normal((40, hk, d)), dt)
+    dx, cu, lens = upload(x), upload(np.array([0, 40], dtype=np.int32)), upload(np.array([10], dtype=np.int32))
+    capi.kv_cache_write(cache, dx.ptr, hk * d, d, dx.ptr, hk * d, d, cu.ptr, lens.ptr, pages.dev["table"].ptr, 3, 1, 40, dt)
+    capi.synchronize()
+    assert capi.kernel_status(0) == 322
+    pages.put(0, 0, x[30:], x[30:])
+    for name in ("k", "v"):
+        assert np.array_equal(pages.dev[name].download(np.uint16, pages.k.shape), getattr(pages, name))
+
+
