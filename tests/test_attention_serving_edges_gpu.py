@@ -393,3 +393,148 @@ def test_tokens_without_a_place_are_not_stored():
         assert np.array_equal(pages.dev[name].download(np.uint16, pages.k.shape), getattr(pages, name))
 
 
+# ---- calls large enough for four heads per lane group --------------------------------------------------
+@pytest.mark.parametrize("dt,hk,d,page,coded,head_major", [
+    (BF, 4, 64, 16, True, True), (FH, 5, 80, 32, True, False), (BF, 7, 128, 64, False, True), (BF, 8, 128, 16, True, True),
+    (FH, 6, 48, 8, False, False), (BF, 8, 96, 128, False, False)])
+def test_large_writes_and_reads_bit_for_bit(dt, hk, d, page, coded, head_major):
+    """Rows x heads x lanes of a row pass two per thread slot of the GPU (2 * 148 * 2048)."""
+    rng = np.random.default_rng(44)
+    rows = -(-2 * 148 * 2048 // (hk * (8 if d <= 64 else 16))) + 37
+    new = [rows // 3, 0, 1, rows - rows // 3 - 1]
+    lens = [new[0] + 11, 5, 40, new[3]]
+    pages = ref.Pages(rng, lens, page, hk, d, dt, coded, head_major, fill=7)
+    cache, cu = pages.upload(), ref.offsets(new)
+    ld = hk * d + 16
+    both = [ref.store(rng.standard_normal((rows, ld)) * np.exp2(rng.integers(-30, 8, (rows, 1))), dt) for _ in range(2)]
+    k, v = (b[:, :hk * d].reshape(rows, hk, d) for b in both)
+    dk, dv, dcu, dlen = upload(both[0]), upload(both[1]), upload(cu), upload(np.array(lens, dtype=np.int32))
+    table, stride = pages.dev["table"].ptr, pages.table.shape[1]
+    capi.kv_cache_write(cache, dk.ptr, ld, d, dv.ptr, ld, d, dcu.ptr, dlen.ptr, table, stride, len(new), rows, dt)
+    capi.synchronize()
+    assert capi.kernel_status(0) == 0
+    for s, n in enumerate(new):
+        pages.put(s, lens[s] - n, k[cu[s]:cu[s + 1]], v[cu[s]:cu[s + 1]])
+    for name in ("k", "v") + (("ks", "vs") if coded else ()):
+        want = getattr(pages, name)
+        assert np.array_equal(pages.dev[name].download(want.dtype, want.shape), want), name
+    keep = [new[0] + 3, 2, 40, new[3]]                       # some of the sequences in part
+    cuk = ref.offsets(keep)
+    total = int(cuk[-1]) + 3
+    old = hk * d + 8
+    outs = [upload(np.full((total, old), FILL, dtype=np.uint16)) for _ in range(2)]
+    dcuk = upload(cuk)
+    capi.kv_cache_read(cache, outs[0].ptr, old, d, outs[1].ptr, old, d, dcuk.ptr, table, stride, len(keep), total, dt)
+    capi.synchronize()
+    assert capi.kernel_status(0) == 0
+    for i, out in enumerate(outs):
+        got = out.download(np.uint16, (total, old))
+        assert np.all(got[cuk[-1]:] == FILL) and np.all(got[:, hk * d:] == FILL)
+        for s, n in enumerate(keep):
+            want = ref.store(pages.values(s, n)[i], dt).reshape(n, hk * d)
+            g = got[cuk[s]:cuk[s + 1], :hk * d]
+            nan = np.isnan(ref.load(want, dt))
+            assert np.array_equal(np.isnan(ref.load(g, dt)), nan) and np.array_equal(g[~nan], want[~nan])
+
+
+# ---- layouts -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt,h,hk,d", [(BF, 8, 2, 64), (FH, 6, 2, 128), (BF, 4, 4, 80)])
+def test_prompts_whose_heads_lie_apart(dt, h, hk, d):
+    """[head, token, dim] instead of [token, head, dim], for every operand."""
+    rng = np.random.default_rng(46)
+    lens = [130, 0, 61]
+    call = Prompt(rng, dt, h, hk, d, lens)
+    rows = sum(lens)
+    q, k, v = (upload(x.transpose(1, 0, 2)) for x in (call.q, call.k, call.v))
+    out, lse = upload(np.full((h, rows + 3, d), FILL, dtype=np.uint16)), capi.DeviceBuffer(rows * h * 4)
+    p = call.p
+    p.q_token_stride = p.k_token_stride = p.v_token_stride = p.o_token_stride = d
+    p.q_head_stride = p.k_head_stride = p.v_head_stride = rows * d
+    p.o_head_stride = (rows + 3) * d
+    capi.attention_prompt(p, q.ptr, k.ptr, v.ptr, out.ptr, call.dcu.ptr, call.dcuk.ptr, lse=lse.ptr)
+    capi.synchronize()
+    assert capi.kernel_status(0) == 0
+    got = out.download(np.uint16, (h, rows + 3, d))
+    assert np.all(got[:, rows:] == FILL)
+    seqs = [(ref.load(call.k[a:b], dt), ref.load(call.v[a:b], dt)) for a, b in zip(call.cu, call.cu[1:])]
+    check_rows(got[:, :rows].transpose(1, 0, 2), lse.download(np.float32, (rows, h)).astype(np.float64), call.q, call.cu, seqs,
+               dt, d, np.float32(call.scale), 1)
+
+
+@pytest.mark.parametrize("lq", [[1, 1, 1], [20, 3, 100]], ids=["decode", "chunk"])
+@pytest.mark.parametrize("dt,h,hk,d,page,coded", [(BF, 8, 2, 16, 8, True), (FH, 4, 2, 48, 8, True), (BF, 8, 2, 128, 8, True),
+                                                  (BF, 8, 2, 128, 8, False), (FH, 8, 2, 32, 8, False), (BF, 6, 2, 112, 512, True),
+                                                  (FH, 32, 2, 16, 16, True)])
+def test_small_pages_and_small_heads(dt, h, hk, d, page, coded, lq):
+    """Query and output rows with their heads apart, lengths that end inside a page and a tile."""
+    rng = np.random.default_rng(47)
+    call = Call(rng, dt, h, hk, d, lq, [1, 267, 777], page=page, coded=coded)
+    rows = call.rows
+    q, out = upload(call.q.transpose(1, 0, 2)), upload(np.full((h, rows, d), FILL, dtype=np.uint16))
+    call.p.q_token_stride = call.p.o_token_stride = d
+    call.p.q_head_stride = call.p.o_head_stride = rows * d
+    call.dq, call.out = q, out
+    call.run()
+    capi.synchronize()
+    assert capi.kernel_status(0) == 0
+    got = out.download(np.uint16, (h, rows, d)).transpose(1, 0, 2)
+    seqs = [tuple(call.pages.values(s, n)) for s, n in enumerate(call.lk)]
+    check_rows(got, call.lse.download(np.float32, (rows, h)).astype(np.float64), call.q, call.cu, seqs, dt, d, np.float32(call.scale),
+               1, coded)
+
+
+@pytest.mark.parametrize("coded", [False, True], ids=["same", "e4m3"])
+def test_writes_and_reads_of_rows_whose_heads_lie_apart(coded):
+    """k and v with strides of their own."""
+    rng = np.random.default_rng(48)
+    dt, hk, d, n = FH, 3, 64, 45
+    pages = ref.Pages(rng, [n], 16, hk, d, dt, coded, True, fill=7)
+    cache = pages.upload()
+    k, v = (ref.store(rng.standard_normal((n, hk, d)), dt) for _ in range(2))
+    dk = upload(k.transpose(1, 0, 2))
+    wide = np.full((n, hk, d + 24), FILL, dtype=np.uint16)
+    wide[..., :d] = v
+    dv, cu, lens = upload(wide), upload(np.array([0, n], dtype=np.int32)), upload(np.array([n], dtype=np.int32))
+    strides = d, n * d, hk * (d + 24), d + 24
+    capi.kv_cache_write(cache, dk.ptr, strides[0], strides[1], dv.ptr, strides[2], strides[3], cu.ptr, lens.ptr, pages.dev["table"].ptr,
+                        pages.table.shape[1], 1, n, dt)
+    capi.synchronize()
+    pages.put(0, 0, k, v)
+    for name in ("k", "v") + (("ks", "vs") if coded else ()):
+        want = getattr(pages, name)
+        assert np.array_equal(pages.dev[name].download(want.dtype, want.shape), want), name
+    ok, ov = upload(np.full((hk, n, d), FILL, dtype=np.uint16)), upload(np.full(wide.shape, FILL, dtype=np.uint16))
+    capi.kv_cache_read(cache, ok.ptr, strides[0], strides[1], ov.ptr, strides[2], strides[3], cu.ptr, pages.dev["table"].ptr,
+                       pages.table.shape[1], 1, n, dt)
+    capi.synchronize()
+    assert capi.kernel_status(0) == 0
+    want_k, want_v = (ref.store(x, dt) for x in pages.values(0, n))
+    assert np.array_equal(ok.download(np.uint16, (hk, n, d)).transpose(1, 0, 2), want_k)
+    got = ov.download(np.uint16, wide.shape)
+    assert np.array_equal(got[..., :d], want_v) and np.all(got[..., d:] == FILL)
+
+
+def test_two_captured_calls_share_a_workspace_in_turn():
+    """A decoding step and a chunk cut into parts, captured apart, replayed one after the other."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(49)
+    calls = [Call(rng, BF, 16, 2, 128, [1, 2], [1500, 900]), Call(rng, FH, 16, 2, 128, [30, 4], [2500, 1100], coded=True)]
+    size = max(c.size for c in calls)
+    assert min(c.size for c in calls) > 4096
+    work = upload(np.zeros(size, dtype=np.uint8))
+    graphs, stream = [], torch.cuda.Stream()
+    for c in calls:
+        c.work, c.size = work, size
+        c.run()
+        capi.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            c.run(torch.cuda.current_stream().cuda_stream)
+        c.out.upload(np.full(c.q.shape, FILL, dtype=np.uint16))
+    with torch.cuda.stream(stream):
+        for i in (0, 1, 1, 0, 1, 0):
+            graphs[i].replay()
+    torch.cuda.synchronize()
+    assert capi.kernel_status(0) == 0
+    for c in calls:
+        c.check()
