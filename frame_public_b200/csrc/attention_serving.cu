@@ -23,8 +23,8 @@ int check_attention_params(const char* what, const fb200_attention_params* p) {
                      "%s: needs head_dim a multiple of 16 up to 128 and at most 64 query heads per kv head (got %lld, %lld)",
                      what, (long long)p->head_dim, (long long)(p->heads / p->kv_heads));
   }
-  if (!(p->scale > 0.0f) || p->scale > 3.0e38f) {
-    return set_error(FB200_INVALID_ARGUMENT, "%s: the score scale must be positive and finite", what);
+  if (!(p->scale > 0.0f) || p->scale > 2.0e38f) {   // times log2(e) it still has to be finite
+    return set_error(FB200_INVALID_ARGUMENT, "%s: the score scale must be positive and at most 2e38", what);
   }
   const int64_t strides[4] = {p->q_token_stride, p->q_head_stride, p->o_token_stride, p->o_head_stride};
   for (int64_t s : strides) {

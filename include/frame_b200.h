@@ -435,7 +435,7 @@ typedef struct fb200_attention_params {
   int64_t max_kv;    /* no sequence has more keys: for scheduling only */
   int64_t q_token_stride, q_head_stride, o_token_stride, o_head_stride;
   int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;   /* prompt only */
-  float scale;       /* > 0 */
+  float scale;       /* > 0, at most 2e38 */
   int causal;
   int dtype;
 } fb200_attention_params;

@@ -14,3 +14,9 @@ def test_paged_refuses_every_workspace_that_is_too_small(change):
     refused(1, "workspace", paged, p, c, size=0)
     refused(1, "workspace", paged, p, c, work=None, size=size)
     refused(1, "workspace", paged, p, c, work=PTR + 16, size=size)
+
+
+@pytest.mark.parametrize("scale", [2.5e38, 3.4e38])
+def test_a_score_scale_whose_exponent_overflows_is_refused(scale):
+    refused(1, "scale", paged, good_params(scale=scale), good_cache())
+    refused(1, "scale", capi.attention_paged_workspace, good_params(scale=scale), good_cache())
