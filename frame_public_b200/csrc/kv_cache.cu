@@ -9,7 +9,7 @@
 // Read: code * 2^e, rounded once, at most the type's largest finite number.
 // Both are bound by HBM: (2 + 1) bytes a number either way, 1/head_dim more for the scales.  A lane group
 // (16 bytes a lane on the dense side) takes four heads of one token: the token's place, a binary search and two
-// dependent loads, is found once for eight vectors in flight (one head a group: TIME_BEFORE).
+// dependent loads, is found once for eight vectors in flight (figures at dispatch_rows).
 #include "kv_cache.cuh"
 
 #include <climits>

@@ -443,7 +443,8 @@ typedef struct fb200_attention_params {
  * t % page_size.  k and v share the strides (elements of `dtype`).  dtype: BF16 / F16, or U8 for
  * e4m3 codes with one scale per (token, kv head): byte b stands for 2^(b - 127), and the values are
  * code * 2^(b - 127); b = 255 makes the whole token-head NaN.  What attention computes from finite
- * e4m3 values stops at the largest finite number of its type.  page_size a power of two from 8 up. */
+ * e4m3 values stops at the largest finite number of its type; where every value that a row sees is
+ * below 2^-72 they lose bits, below 2^-83 the row becomes 0.  page_size a power of two from 8 up. */
 typedef struct fb200_kv_cache {
   void* k;
   void* v;

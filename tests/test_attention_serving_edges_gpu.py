@@ -231,14 +231,14 @@ def score_error(arg, d):
     return (d + 8) * 2.0 ** -23 * arg + 2.0 ** -20
 
 
-def small_weights_bound(o, mag, arg, dt, d, n, weights, values):
+def small_weights_bound(o, mag, arg, dt, d, n, weights, values, smallest=2.0 ** -24):
     """Probabilities are held in float16 for float16 and e4m3 caches, the largest as 2^7 or more: half a step
     is 2^-11 of a probability, and at least 2^-25, which is 2^-32 of the row's largest weight.  (`weights`:
     that largest one per row, p times the value's scale; `values`: the sum over the keys of what it is
     multiplied with, codes or numbers.)  A score is an fp32 sum of d products, as in ref.bounds; O and the row
     sum grow in fp32 by 16 keys at a time or more, each addition truncated at worst."""
     delta, steps = score_error(arg, d), n / 16 * 2.0 ** -23
-    return (2.0 ** -11 + 2 * delta[..., None] + 2 * steps) * mag + ref.UNIT[dt] * np.abs(o) + 2.0 ** -24 + 2.0 ** -32 * weights * values
+    return (2.0 ** -11 + 2 * delta[..., None] + 2 * steps) * mag + ref.UNIT[dt] * np.abs(o) + smallest + 2.0 ** -32 * weights * values
 
 
 @pytest.mark.parametrize("form,dt,coded", [("prompt", FH, False)] +
@@ -302,6 +302,27 @@ def test_probabilities_over_an_e4m3_cache_keep_the_bits_of_float16(dt, d, lq):
     codes = (np.abs(vv) * 2.0 ** -e[..., None]).sum(0).repeat(h // hk, 0)                           # [h, d]
     tol = small_weights_bound(o, mag, arg, dt, d, n, 2.0 ** e.max(), codes)
     assert np.all(np.abs(got - o) <= tol), float(np.max(np.abs(got - o) / tol))
+
+
+@pytest.mark.parametrize("lq", [1, 3, 20], ids=["decode", "draft", "chunk"])
+@pytest.mark.parametrize("gain", [2.0 ** -40, 2.0 ** -66, 2.0 ** 100])
+def test_values_of_any_size_keep_their_bits_over_an_e4m3_cache(gain, lq):
+    """Scales from below the smallest one that rows are normalised with (2^-60) to large ones."""
+    rng = np.random.default_rng(50)
+    n, h, hk, d, dt = 500, 8, 2, 64, BF
+    call = Call(rng, dt, h, hk, d, [lq], [n], coded=True)
+    call.pages.put(0, 0, ref.store(rng.standard_normal((n, hk, d)), dt), ref.store(rng.standard_normal((n, hk, d)) * gain, dt))
+    resend(call)
+    got, _ = run(call)
+    kk, vv = call.pages.values(0, n)
+    o, l, mag, arg = ref.attention(ref.load(call.q, dt), kk, vv, np.float32(call.scale), True)
+    e = np.maximum(call.pages.vs[call.pages._at(call.pages.vs, 0, np.arange(n))].astype(np.float64) - 127, -60)
+    codes = (np.abs(vv) / gain).sum(0).repeat(h // hk, 0) * gain / 2.0 ** e.min()                   # at least the sum of them
+    # without the term for float16's smallest numbers, which the result's bfloat16 does not have (adding 2^-24 and
+    # taking it away again would leave a multiple of 2^-76 of a bound near 2^-78)
+    tol = small_weights_bound(o, mag, arg, dt, d, n, 2.0 ** e.max(), codes, 0.0)
+    assert np.all(np.abs(got - o) <= tol), float(np.max(np.abs(got - o) / tol))
+    assert np.median(tol / np.abs(o)) < 0.05
 
 
 @pytest.mark.parametrize("lq,n", [(1, 100), (20, 100)], ids=["decode", "chunk"])
