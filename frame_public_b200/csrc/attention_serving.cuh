@@ -32,10 +32,12 @@ __device__ __forceinline__ void serving_lengths(const ServingProblem& p, const P
 }
 
 // Whether serving_lengths takes those of sequence s as they are.  keys: kv_len where PAGED, else cu_kv, and
-// most_keys what they are cut to.
+// most_keys what they are cut to.  The keys of a sequence without rows (an empty place of a padded batch) may be
+// anything.
 template <bool PAGED>
 __device__ __forceinline__ bool lengths_fit(const int32_t* cu_q, const int32_t* keys, int s, int q_rows, int most_keys) {
   if (!span_fits(cu_q, s, q_rows)) return false;
+  if (cu_q[s] == cu_q[s + 1]) return true;
   if constexpr (PAGED) return keys[s] >= 0 && keys[s] <= most_keys;
   else return span_fits(keys, s, most_keys);
 }

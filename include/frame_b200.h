@@ -426,7 +426,7 @@ FB200_API int fb200_attention_fan(const void* q_base, int64_t q_rows, int64_t q_
  * multiple of 16 up to 128; heads a multiple of kv_heads, heads / kv_heads <= 64.  Anything else
  * is FB200_UNIMPLEMENTED or FB200_INVALID_ARGUMENT.  q_rows and the other extents bound every access:
  * offsets and lengths that leave them (negative, falling, past the rows or the table) are cut to them and
- * recorded as kernel status 322.  All pointers belong to the current device. */
+ * recorded as kernel status 322 (not the keys of a sequence without query rows).  All pointers belong to the current device. */
 typedef struct fb200_attention_params {
   int64_t n_seqs, heads, kv_heads, head_dim;
   int64_t q_rows;    /* rows of q and o */

@@ -365,6 +365,16 @@ def test_lengths_that_are_cut_are_recorded(lq, what, cu, lens):
                np.float32(call.scale), 1)
 
 
+@pytest.mark.parametrize("lq", [[1, 0, 1, 0, 0], [20, 0, 30, 0, 0]], ids=["decode", "chunk"])
+def test_empty_places_of_a_padded_batch_are_not_recorded(lq):
+    """A captured step keeps its number of sequences: places without rows, whose length is not looked at."""
+    rng = np.random.default_rng(51)
+    call = Call(rng, BF, 8, 2, 64, lq, [100, 0, 300, 0, 0])
+    call.dlen.upload(np.array([100, -1, 300, 1 << 30, -1], dtype=np.int32))
+    run(call, 0)
+    call.check()
+
+
 @pytest.mark.parametrize("cu,cuk", [([0, 40, 1 << 28], None), ([-1, 40, 70], None), (None, [0, 40, 71]), (None, [0, 60, 40])])
 def test_prompt_offsets_that_are_cut_are_recorded(cu, cuk):
     rng = np.random.default_rng(41)
